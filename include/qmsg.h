@@ -271,6 +271,65 @@ int qmsg_layer_norm(qmsg_ctx *ctx, int layer, const float *w);
 /* Wait for everything enqueued on the context's stream. */
 int qmsg_sync(qmsg_ctx *ctx);
 
+/* ------------------------------------------------------------------ attention ---- */
+
+/* What stands between the trunk's q/k/v and output products (attention, src/model.c:428-497) on
+ * device rows: the norm of each query and key head, the rotation (rope_neox, src/model.c:412-422), a
+ * paged cache of keys and values, and causal attention over it with grouped heads. Activations are
+ * fp32; sums, norms and the softmax are formed in fp32 (fp16 caches: products of the cached values
+ * with queries and weights of 22 bits). The reference's sums run in another order: results agree to
+ * rounding, not bit for bit.
+ *
+ * Order of calls, per step: qmsg_attn_batch with the sequences' lengths and page tables, then for
+ * each layer qmsg_attn_append_device and qmsg_attn_device. */
+typedef struct {
+    int n_head, n_head_kv;      /* query heads, a multiple of the kv heads; at most 1024              */
+    int head_dim;               /* D: 64 or 128                                                        */
+    int type;                   /* of the cache: QMSG_T_F16 or QMSG_T_F32 (the reference's)            */
+    int page_tokens;            /* tokens of a page: 16, 32, 64, 128 or 256                            */
+    int n_page;                 /* pages of each layer                                                 */
+    int n_layer;
+    int max_seq, max_tokens;    /* most sequences and new tokens of a batch                            */
+    int max_pages;              /* most pages of a sequence                                            */
+    int qk_norm;                /* 1: heads are normed before the rotation (qmsg_attn_norms)           */
+    float rope_base;            /* rotation by position * rope_base^(-2 i / D), element i with i + D/2 */
+    float scale;                /* of the scores; 0: 1 / sqrt(D)                                       */
+} qmsg_attn_cfg;
+
+/* Bytes of a cache's keys, and as many of its values; 0 for a configuration that is not taken. */
+uint64_t qmsg_attn_cache_bytes(const qmsg_attn_cfg *cfg);
+
+/* A cache and what its calls need (plans, workspace), freed with the context; *id names it. d_k and d_v:
+ * the caller's device memory for keys and values (qmsg_attn_cache_bytes each, 16-byte aligned,
+ * several may share it), or both NULL: the context's. Pages of keys are [kv head][slot][D], pages
+ * of values [kv head][D][slot], layer by layer. Slots that hold no token yet may hold anything. */
+int qmsg_attn_create(qmsg_ctx *ctx, const qmsg_attn_cfg *cfg, void *d_k, void *d_v, int *id);
+int qmsg_attn_cache(qmsg_ctx *ctx, int id, void **d_k, void **d_v);
+
+/* A layer's attn_q_norm and attn_k_norm, head_dim host floats each; NULL: unit weights (the default). */
+int qmsg_attn_norms(qmsg_ctx *ctx, int id, int layer, const float *q_norm, const float *k_norm);
+
+/* The sequences of the next calls (host arrays, read before the call returns): sequence i has kv_len[i]
+ * tokens, the last q_len[i] of them new, on pages[i * stride + 0 ..]. The rows of device buffers are the
+ * new tokens, sequence by sequence. A sequence may have no new token. Neighbouring sequences whose
+ * tables start with the same pages have those read once for all. Everything is checked before anything
+ * changes: a page id outside the cache, a page that would take new tokens twice, or more than the maxima
+ * is QMSG_E_INVALID, and the batch stays what it was. Not while the stream is capturing; calls
+ * captured into a graph work on the batch that is set when the graph is replayed (replay on
+ * qmsg_stream(ctx), or ordered with it). */
+int qmsg_attn_batch(qmsg_ctx *ctx, int id, int n_seq, const int *q_len, const int *kv_len, const int32_t *pages, int stride);
+
+/* For the batch's T new tokens, all on device buffers (16-byte aligned): norm and rotate the query heads
+ * d_q [T][n_head][D] into d_qr (which may be d_q; both NULL: keys and values only), and write the
+ * normed and rotated keys d_k [T][n_head_kv][D] and the values d_v into the cache at the tokens'
+ * positions. Enqueued without waiting. */
+int qmsg_attn_append_device(qmsg_ctx *ctx, int id, int layer, float *d_qr, const float *d_q, const float *d_k, const float *d_v, float eps);
+
+/* d_out [T][n_head][D] = softmax(scale q K^T) V over the cache for the batch's new tokens, each seeing its
+ * sequence's positions up to its own. d_q [T][n_head][D] is read as it is; d_out must not overlap it.
+ * Enqueued without waiting. */
+int qmsg_attn_device(qmsg_ctx *ctx, int id, int layer, const float *d_q, float *d_out);
+
 /* ------------------------------------------------------------------ device buffers ---- */
 
 /* No reference counterpart: device memory owned by the context (freed by qmsg_destroy). */
@@ -325,7 +384,7 @@ int qmsg_eval_exp(qmsg_ctx *ctx, const double *x, int n, double *out);
  * every kernel launch of the context is bracketed by an event pair. */
 int qmsg_profile(qmsg_ctx *ctx, int enable);
 /* Launch count and summed milliseconds of kernel `name` since profiling was enabled
- * (synchronises the stream). Names: "route", "gateup", "down", and the MFMA-path kernels. */
+ * (synchronises the stream). Names: "route", "gateup", "down", the MFMA-path kernels, "append", "attend", "join". */
 int qmsg_profile_read(qmsg_ctx *ctx, const char *name, int64_t *launches, double *total_ms);
 
 /* No reference counterpart: a plain device copy of `bytes` (multiple of 16) with a simple

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/qmsg.h"
+#include "qmsg_ctx.h"
 #include "qmsg_gguf.h"
 #include "qmsg_internal.h"
 #include "qmsg_synth.h"
@@ -18,27 +19,6 @@
 using namespace qmsg;
 
 namespace {
-
-struct LayerStore {
-    float *router = nullptr;
-    float *norm = nullptr;        /* ffn_norm [E], nullptr: unit weights */
-    uint8_t *gate = nullptr, *up = nullptr, *down = nullptr;
-    int gate_type = -1, up_type = -1, down_type = -1;
-    bool ready = false;
-};
-
-/* A dense (trunk) matrix resident in HBM, QmsMat (src/quant.h:11-16) with device data. */
-struct DenseStore {
-    uint8_t *w = nullptr;
-    int type = -1;
-    int64_t rows = 0, cols = 0;
-    uint64_t rb = 0;
-};
-
-struct ProfRec {
-    std::string name;
-    hipEvent_t a, b;
-};
 
 /* qms_row_bytes (src/gguf.c:85-96). */
 uint64_t row_bytes(int type, int64_t ne0)
@@ -128,36 +108,7 @@ size_t scratch_carve(const qmsg_cfg &cfg, size_t T, uint8_t *base, size_t cap, S
 
 }  // namespace
 
-struct qmsg_ctx {
-    int device = 0;
-    qmsg_cfg cfg{};
-    int n_layer = 0, max_tokens = 0, path = QMSG_PATH_AUTO;
-    int norm_walk = 0;                      /* rmsnorm: form every row's sum in order */
-    unsigned long long *d_walked = nullptr; /* rmsnorm: rows that formed it in order */
-    float *d_hb = nullptr;                  /* the one-token chain's second row of h */
-    int n_cu = 256;
-    hipStream_t stream = nullptr;
-    std::vector<LayerStore> layers;
-    Scratch S{};
-    std::vector<void *> scratch_allocs, user_allocs;
-    float *d_x = nullptr, *d_out = nullptr;
-    std::vector<DenseStore> mats;
-    /* grow-on-demand buffers of the dense products: input records, host-call staging */
-    void *dense_xqk = nullptr;
-    size_t dense_xqk_bytes = 0;
-    bool dense_xqk_held = false;            /* by a captured call: never freed before the context */
-    void *dense_io = nullptr;
-    size_t dense_io_bytes = 0;
-    /* pinned rows of the host-buffer layer call (kHostStage bytes in, as many out), on first use */
-    uint8_t *pin = nullptr;
-    std::string err;
-    bool prof = false;
-    std::vector<ProfRec> prof_recs, prof_free;
-    struct Tot { std::string name; int64_t n; double ms; };
-    std::vector<Tot> prof_tot;
-};
-
-static int fail(qmsg_ctx *c, int code, const char *fmt, ...)
+int qmsg::fail(qmsg_ctx *c, int code, const char *fmt, ...)
 {
     char buf[512];
     va_list ap;
@@ -169,18 +120,7 @@ static int fail(qmsg_ctx *c, int code, const char *fmt, ...)
     return code;
 }
 
-/* A failed runtime call's error also stays the thread's last error, which the next launch would
- * report as its own: it is cleared where the failure is returned or absorbed. */
-#define HIP_TRY(c, call)                                                                               \
-    do {                                                                                               \
-        hipError_t e_ = (call);                                                                        \
-        if (e_ != hipSuccess) {                                                                        \
-            (void)hipGetLastError();                                                                   \
-            return fail((c), QMSG_E_DEVICE, "%s: %s", #call, hipGetErrorString(e_));                   \
-        }                                                                                              \
-    } while (0)
-
-static int dev_alloc(qmsg_ctx *c, void **p, size_t bytes, std::vector<void *> &list)
+int qmsg::dev_alloc(qmsg_ctx *c, void **p, size_t bytes, std::vector<void *> &list)
 {
     /* 256 bytes of tail padding: kernels may read one aligned word past a tensor's end. */
     hipError_t e = hipMalloc(p, bytes + 256);
@@ -193,7 +133,7 @@ static int dev_alloc(qmsg_ctx *c, void **p, size_t bytes, std::vector<void *> &l
 }
 
 /* Timing hook: hands out an event pair per kernel dispatch while profiling is on. */
-static void prof_events(void *vc, const char *kernel, hipEvent_t *start, hipEvent_t *stop)
+void qmsg::prof_events(void *vc, const char *kernel, hipEvent_t *start, hipEvent_t *stop)
 {
     qmsg_ctx *c = (qmsg_ctx *)vc;
     ProfRec r;
@@ -208,15 +148,6 @@ static void prof_events(void *vc, const char *kernel, hipEvent_t *start, hipEven
     *start = r.a;
     *stop = r.b;
 }
-
-#define LAUNCH(c, name, expr)                                                                             \
-    do {                                                                                                  \
-        const LaunchTimer timer_{ (c), prof_events };                                                     \
-        g_launch_timer = (c)->prof ? &timer_ : nullptr;                                                   \
-        hipError_t e_ = (expr);                                                                           \
-        g_launch_timer = nullptr;                                                                         \
-        if (e_ != hipSuccess) return fail((c), QMSG_E_DEVICE, "%s launch: %s", (name), hipGetErrorString(e_)); \
-    } while (0)
 
 extern "C" {
 
@@ -294,6 +225,7 @@ void qmsg_destroy(qmsg_ctx *c)
         hipFree(L.down);
     }
     for (auto &m : c->mats) hipFree(m.w);
+    for (auto &a : c->attns) attn_release(*a);
     hipFree(c->dense_xqk);
     hipFree(c->dense_io);
     if (c->pin) hipHostFree(c->pin);

@@ -1,0 +1,761 @@
+/* qmsg_attn.hip - head norms, rotation and the append to the paged cache; attention over the cache.
+ *
+ * Cache pages: keys [kv head][slot][D], values [kv head][D][slot], so that both products read their
+ * matrix operand in 16-byte pieces along the axis they sum over, without a transpose:
+ *
+ *   S^T = K q^T     (keys x rows),  A operand 16 keys x D,      B operand the rows' queries
+ *   O^T += V^T P^T  (D x rows),     A operand 16 d x the keys,  B operand P^T
+ *
+ * A 16x16 result leaves lane (col = lane % 16, g = lane / 16) the four keys 4g .. 4g+3 of row col,
+ * and the B operand wants from it one 16-byte piece of consecutive keys. The order in which keys
+ * are dealt to the rows of the first product is free, so key (m / 4) * CE + 4 tl + m % 4 of a step goes
+ * to row m of its tile tl: then lane (col, g) holds exactly the keys g * CE .. of its row, and P needs
+ * neither a shuffle nor LDS on its way into the second product (CE elements in 16 bytes: 8 f16 in
+ * two tiles a step of 32 keys, 4 f32 in one tile of 16).
+ *
+ * Activations are fp32. With an f16 cache q (scaled by a power of two so that its largest element
+ * lies in [2^8, 2^9)) and p are split into two f16, x = hi + lo to 22 bits, and each product is two f16 MFMAs
+ * into fp32: twice the f16 work, against the sixteenth of the rate that fp32 MFMAs would have. An fp32
+ * cache takes the fp32 MFMAs as it is.
+ *
+ * Softmax in one pass: p = 2^(c s - ref) with ref a row's running reference, set 6 below the row's
+ * largest score so far and raised only when a score passes it by 14, so that p stays below 2^14 (f16's
+ * range) and the usual step needs no reduction across lanes. Sums, references and O are fp32. */
+#include <cmath>
+
+#include "qmsg_attn.h"
+#include "qmsg_device.h"
+
+namespace qmsg {
+
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLowest = -INFINITY;
+
+/* A cache of one type and head width. */
+template <int TYPE, int D>
+struct Att {
+    static constexpr int ES = TYPE == 1 ? 2 : 4;        /* bytes of an element                    */
+    static constexpr int CE = 16 / ES;                  /* elements of a piece                    */
+    static constexpr int TL = CE / 4;                   /* key tiles of a step                    */
+    static constexpr int KS = 16 * TL;                  /* keys of a step                         */
+    static constexpr int NCH = D / (4 * CE);            /* pieces per lane of a key tile          */
+    static constexpr int NK = TL * NCH, NV = D / 16;    /* 16-byte loads per lane and step        */
+};
+
+/* The row's query as B operand: lane (col, g) holds d = 4 CE c + CE g .. of piece c. */
+template <int TYPE, int D>
+struct AttQ {
+    h8 hi[Att<TYPE, D>::NCH], lo[Att<TYPE, D>::NCH];
+};
+template <int D>
+struct AttQ<0, D> {
+    f32x4 v[Att<0, D>::NCH];
+};
+
+/* Running softmax of a lane's row: reference, this lane's part of the sum, O^T (d = 16 i + 4 g + r). */
+template <int D>
+struct AttRow {
+    float ref, l;
+    f32x4 o[D / 16];
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+/* The larger of the four lanes of a row (g = 0..3), in all of them. */
+__device__ __forceinline__ float row_max(float v)
+{
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+    u = __builtin_bit_cast(uint32_t, v);
+    r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float row_sum(float v)
+{
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    u = __builtin_bit_cast(uint32_t, v);
+    r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+/* Load a row's query; returns what its scores are multiplied with to stand in powers of two. */
+template <int TYPE, int D>
+__device__ __forceinline__ float load_q(const float *row, bool any, int g, float scale_log2, AttQ<TYPE, D> &q)
+{
+    using A = Att<TYPE, D>;
+    if constexpr (TYPE == 0) {
+#pragma unroll
+        for (int c = 0; c < A::NCH; c++) q.v[c] = any ? *(const f32x4 *)(row + 16 * c + 4 * g) : f32x4{ 0, 0, 0, 0 };
+        return scale_log2;
+    } else {
+        f32x4 x[A::NCH][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < A::NCH; c++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                x[c][j] = any ? *(const f32x4 *)(row + 32 * c + 8 * g + 4 * j) : f32x4{ 0, 0, 0, 0 };
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[c][j][e]));
+            }
+        top = row_max(top);
+        /* a row of zeros, of subnormals only or with an infinity keeps a scale inside fp32's range */
+        const int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+        const int sh = ex < -110 || ex > 127 ? 0 : 8 - ex;
+        const float up = __builtin_bit_cast(float, (uint32_t)(127 + sh) << 23), down = __builtin_bit_cast(float, (uint32_t)(127 - sh) << 23);
+#pragma unroll
+        for (int c = 0; c < A::NCH; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = x[c][e / 4][e % 4] * up;
+                const _Float16 hi = (_Float16)v;
+                q.hi[c][e] = hi;
+                q.lo[c][e] = (_Float16)(v - (float)hi);
+            }
+        return scale_log2 * down;
+    }
+}
+
+/* One step's scores of NT row tiles: s[n][tl][r] of key g * CE + 4 tl + r. key(tl, c): the lane's piece. */
+template <int TYPE, int D, int NT, class K>
+__device__ __forceinline__ void scores(K key, const AttQ<TYPE, D> (&q)[NT], f32x4 (&s)[NT][Att<TYPE, D>::TL])
+{
+    using A = Att<TYPE, D>;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int t = 0; t < A::TL; t++) s[n][t] = f32x4{ 0, 0, 0, 0 };
+#pragma unroll
+    for (int c = 0; c < A::NCH; c++)
+#pragma unroll
+        for (int t = 0; t < A::TL; t++) {
+            const u32x4 k = key(t, c);
+            if constexpr (TYPE == 0) {
+                const f32x4 x = __builtin_bit_cast(f32x4, k);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[n].v[c][e], s[n][t], 0, 0, 0);
+            } else {
+                const h8 x = __builtin_bit_cast(h8, k);
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].lo[c], s[n][t], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].hi[c], s[n][t], 0, 0, 0);
+            }
+        }
+}
+
+/* P as B operand. */
+template <int TYPE>
+struct AttP {
+    h8 hi, lo;
+};
+template <>
+struct AttP<0> {
+    f32x4 v;
+};
+
+/* A row's step of the softmax: keys from `limit` on are hidden (left: limit less the lane's first key). */
+template <int TYPE, int D, bool MASK>
+__device__ __forceinline__ void soften(float c, int left, f32x4 (&s)[Att<TYPE, D>::TL], AttRow<D> &row, AttP<TYPE> &p)
+{
+    using A = Att<TYPE, D>;
+    if constexpr (MASK) {
+#pragma unroll
+        for (int t = 0; t < A::TL; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[t][r] = 4 * t + r < left ? s[t][r] : kLowest;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < A::TL; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) top = fmaxf(top, s[t][r]);
+    top *= c;
+    if (__builtin_expect(__ballot(top > row.ref + 14.0f) != 0, 0)) {
+        const float ref = fmaxf(row.ref, row_max(top) - 6.0f);
+        const float a = ref == row.ref ? 1.0f : exp2_fast(row.ref - ref);
+        row.ref = ref;
+        row.l *= a;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) row.o[i] *= a;
+    }
+    const float nref = row.ref == kLowest ? 0.0f : -row.ref;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < A::TL; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], c, nref));
+            sum += s[t][r];
+        }
+    row.l += sum;
+    if constexpr (TYPE == 0) {
+        p.v = s[0];
+    } else {
+#pragma unroll
+        for (int t = 0; t < A::TL; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                /* hi rounds towards zero: what it drops is in lo, to 11 more bits */
+                const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(s[t][r], s[t][r + 1]));
+                const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(s[t][r] - (float)hi.x, s[t][r + 1] - (float)hi.y));
+                p.hi[4 * t + r] = hi.x;
+                p.hi[4 * t + r + 1] = hi.y;
+                p.lo[4 * t + r] = lo.x;
+                p.lo[4 * t + r + 1] = lo.y;
+            }
+    }
+}
+
+/* Masks over the lane's piece of values: keys the item has (of n_key from the piece's first on), and of
+ * those the ones that not every row sees (from n_full on). */
+struct AttMask {
+    uint32_t has[4], some[4];
+};
+template <int TYPE>
+__device__ __forceinline__ AttMask piece_mask(int n_full, int n_key)
+{
+    AttMask m;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        if constexpr (TYPE == 0) {
+            m.has[w] = w < n_key ? ~0u : 0u;
+            m.some[w] = w >= n_full ? m.has[w] : 0u;
+        } else {
+            m.has[w] = (2 * w < n_key ? 0xffffu : 0u) | (2 * w + 1 < n_key ? 0xffff0000u : 0u);
+            m.some[w] = m.has[w] & ((2 * w >= n_full ? 0xffffu : 0u) | (2 * w + 1 >= n_full ? 0xffff0000u : 0u));
+        }
+    }
+    return m;
+}
+
+/* The piece with zeros for keys past the item's end (what a page holds there may be anything), and for
+ * infinities and NaN of keys that some rows do not see: 0 * infinity would reach these. The rows that do
+ * see them get them in the end (add_wild). */
+template <int TYPE>
+__device__ __forceinline__ u32x4 clean(u32x4 v, const AttMask &m, uint32_t &bad)
+{
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        uint32_t wild;                                  /* all ones where the exponent is */
+        if constexpr (TYPE == 0) {
+            wild = (uint32_t)((int32_t)((v[w] & 0x7f800000u) + 0x00800000u) >> 31);
+        } else {
+            const uint32_t b = ((v[w] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+            wild = (b - (b >> 15)) | b;
+        }
+        wild &= m.some[w];
+        bad |= wild;
+        v[w] &= m.has[w] & ~wild;
+    }
+    return v;
+}
+
+/* O^T += V^T P^T for NT row tiles. V(i): the lane's piece of values d = 16 i + col. */
+template <int TYPE, int D, int NT, class V>
+__device__ __forceinline__ void weigh(V val, const AttP<TYPE> (&p)[NT], AttRow<D> (&row)[NT])
+{
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+        const u32x4 v = val(i);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            if constexpr (TYPE == 0) {
+                const f32x4 x = __builtin_bit_cast(f32x4, v);
+#pragma unroll
+                for (int e = 0; e < 4; e++) row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[n].v[e], row[n].o[i], 0, 0, 0);
+            } else {
+                const h8 x = __builtin_bit_cast(h8, v);
+                row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[n].hi, row[n].o[i], 0, 0, 0);
+                row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[n].lo, row[n].o[i], 0, 0, 0);
+            }
+        }
+    }
+}
+
+/* Byte address of a page's keys or values of one kv head. */
+__device__ __forceinline__ const uint8_t *page_at(const uint8_t *pool, int page, uint32_t page_bytes, uint32_t head_off)
+{
+    return pool + (size_t)(uint32_t)page * page_bytes + head_off;
+}
+
+/* What clean() left out of the keys [from, to) of values d .. d+3, summed. */
+template <int TYPE, int D>
+__device__ __forceinline__ f32x4 wild_sum(const uint8_t *pool, const int32_t *tab, uint32_t page_bytes, uint32_t head_off, int shift, int from,
+                                          int to, int d)
+{
+    constexpr int ES = Att<TYPE, D>::ES;
+    f32x4 sum = { 0, 0, 0, 0 };
+#pragma unroll 1
+    for (int k = from; k < to; k++) {
+        const uint8_t *base = page_at(pool, tab[k >> shift], page_bytes, head_off);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint32_t off = ((uint32_t)(d + r) << shift) + (uint32_t)(k & ((1 << shift) - 1));
+            float v;
+            if constexpr (TYPE == 0) v = *(const float *)(base + off * ES);
+            else v = (float)*(const _Float16 *)(base + off * ES);
+            if (!(fabsf(v) < INFINITY)) sum[r] += v;
+        }
+    }
+    return sum;
+}
+
+/* The part of a call's header that is in use: the launch's own, or the blob's for a captured call. */
+__device__ __forceinline__ const AttnHdr &header(const AttnCall &a) { return a.live ? *(const AttnHdr *)a.blob : a.h; }
+
+/* Where a row's results go: the output where the token has no other part, else its part. */
+__device__ __forceinline__ float *row_out(const AttnCall &a, const AttnTok &tk, int part, int t, int head, int D)
+{
+    return tk.parts == 1 ? a.out + ((size_t)t * a.heads + head) * D : a.part_o + ((size_t)(tk.part + part) * a.heads + head) * D;
+}
+/* A part's reference is +infinity where its sum is NaN, so that joining keeps it. */
+__device__ __forceinline__ void put_row(const AttnCall &a, const AttnTok &tk, int part, int t, int head, int d, int D, float ref, float l,
+                                        f32x4 o, bool stats)
+{
+    const bool whole = tk.parts == 1;
+    *(f32x4 *)(row_out(a, tk, part, t, head, D) + d) = whole ? o * (1.0f / l) : o;
+    if (!whole && stats) {
+        float *ml = a.part_ml + 2 * ((size_t)(tk.part + part) * a.heads + head);
+        ml[0] = l != l ? INFINITY : ref;
+        ml[1] = l;
+    }
+}
+
+/* Few rows (16): eight waves take every eighth step of the item's keys, each from memory straight
+ * into the operands' registers with the next step's loads in flight, and join in LDS. */
+constexpr int kFewWaves = 8;
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
+{
+    using A = Att<TYPE, D>;
+    constexpr int NT = 1;
+    __shared__ __align__(16) float s_o[kFewWaves][16][D + 4];
+    __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
+    const AttnHdr &h = header(a);
+    const int n_item = h.n_work[kAttnFew] * a.kv_heads;
+    const AttnWork *work = (const AttnWork *)(a.blob + h.work[kAttnFew]);
+    const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
+    for (int item = blockIdx.x; item < n_item; item += gridDim.x) {
+        const AttnWork w = work[item / a.kv_heads];
+        const int kvh = item % a.kv_heads;
+        const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
+        const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
+        AttQ<TYPE, D> q[NT];
+        AttRow<D> row[NT];
+        float c[NT];
+        int limit[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int r = w.row + 16 * n + col;
+            const bool any = 16 * n + col < w.rows;
+            const int t = any ? r / a.group : w.row / a.group;
+            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
+            c[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
+            row[n].ref = kLowest;
+            row[n].l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) row[n].o[i] = f32x4{ 0, 0, 0, 0 };
+        }
+        const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
+        const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
+        u32x4 kf[A::NK], vf[A::NV];
+        int kp = 0, vp = 0;
+        uint32_t bad = 0;
+        auto pages = [&](int s) {
+            const int k = w.key0 + s * A::KS;
+            kp = tab[min(k + k_off, last) >> a.shift];
+            vp = tab[min(k + v_off, last) >> a.shift];
+        };
+        auto load_k = [&](int s) {
+            const int slot = (w.key0 + s * A::KS + k_off) & P1;
+            const uint8_t *p = page_at(a.k, kp, a.page_bytes, head_off) + (uint32_t)(slot * D + g * A::CE) * A::ES;
+#pragma unroll
+            for (int t = 0; t < A::TL; t++)
+#pragma unroll
+                for (int i = 0; i < A::NCH; i++) kf[t * A::NCH + i] = *(const u32x4 *)(p + (4 * t * D + 4 * i * A::CE) * A::ES);
+        };
+        auto load_v = [&](int s) {
+            const int slot = (w.key0 + s * A::KS + v_off) & P1;
+            const uint8_t *p = page_at(a.v, vp, a.page_bytes, head_off) + (uint32_t)((col << a.shift) + slot) * A::ES;
+            const uint32_t step = (uint32_t)(16 * A::ES) << a.shift;
+#pragma unroll
+            for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(p + i * step);
+        };
+        if (wave < n_step) {
+            pages(wave);
+            load_k(wave);
+            load_v(wave);
+            if (wave + kFewWaves < n_step) pages(wave + kFewWaves);
+        }
+        for (int s = wave; s < n_step; s += kFewWaves) {
+            const int key = w.key0 + s * A::KS;
+            const bool more = s + kFewWaves < n_step, mask = key + A::KS > w.full;
+            f32x4 sc[NT][A::TL];
+            scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, sc);
+            if (more) load_k(s + kFewWaves);
+            AttP<TYPE> p[NT];
+            if (mask) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) soften<TYPE, D, true>(c[n], limit[n] - key - v_off, sc[n], row[n], p[n]);
+                const AttMask m = piece_mask<TYPE>(w.full - key - v_off, w.key1 - key - v_off);
+#pragma unroll
+                for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; n++) soften<TYPE, D, false>(c[n], 0, sc[n], row[n], p[n]);
+            }
+            weigh<TYPE, D, NT>([&](int i) { return vf[i]; }, p, row);
+            if (more) {
+                load_v(s + kFewWaves);
+                if (s + 2 * kFewWaves < n_step) pages(s + 2 * kFewWaves);
+            }
+        }
+        const bool wild = __syncthreads_or(bad != 0);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float l = row_sum(row[n].l);
+            if (g == 0) {
+                s_m[wave][col] = l != l ? INFINITY : row[n].ref;
+                s_l[wave][col] = l;
+            }
+            __syncthreads();
+            float m = s_m[0][col];
+#pragma unroll
+            for (int i = 1; i < kFewWaves; i++) m = fmaxf(m, s_m[i][col]);
+            const float mine = l != l ? INFINITY : row[n].ref;
+            const float f = mine == kLowest ? 0.0f : exp2_fast(mine - m);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) *(f32x4 *)&s_o[wave][col][16 * i + 4 * g] = row[n].o[i] * f;
+            __syncthreads();
+            for (int e = threadIdx.x; e < 16 * (D / 4); e += 64 * kFewWaves) {
+                const int rr = e / (D / 4), d = e % (D / 4) * 4;
+                if (16 * n + rr >= w.rows) continue;
+                float mm = s_m[0][rr], ll = 0.0f;
+#pragma unroll
+                for (int i = 1; i < kFewWaves; i++) mm = fmaxf(mm, s_m[i][rr]);
+                f32x4 o = { 0, 0, 0, 0 };
+#pragma unroll
+                for (int i = 0; i < kFewWaves; i++) {
+                    const float mi = s_m[i][rr];
+                    ll += mi == kLowest ? 0.0f : exp2_fast(mi - mm) * s_l[i][rr];
+                    o += *(const f32x4 *)&s_o[i][rr][d];
+                }
+                const int r = w.row + 16 * n + rr, t = r / a.group;
+                if (__builtin_expect(wild, 0))
+                    o += wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, min(toks[t].pos + 1, w.key1), d);
+                put_row(a, toks[t], w.part, t, kvh * a.group + r % a.group, d, D, mm, ll, o, d == 0);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+/* Many rows (128): four waves of 32 rows each share tiles of keys and values, copied to LDS by the LDS
+ * DMA, the next tile's copy in flight while one is worked on. Pieces are stored with their index in
+ * the row xored by the row, so that the 16 rows a wave instruction reads lie in all banks. */
+constexpr int kManyThreads = 256;
+
+template <int TYPE, int D>
+struct ManyLds {
+    static constexpr int KT = 2 * Att<TYPE, D>::KS;                 /* keys of a tile             */
+    static constexpr int BYTES = KT * D * Att<TYPE, D>::ES;         /* of its keys, or its values */
+};
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
+{
+    using A = Att<TYPE, D>;
+    using L = ManyLds<TYPE, D>;
+    constexpr int NT = 2, RC = D / A::CE, VC = L::KT / A::CE, NG = L::KT / 16;
+    constexpr int NL = L::BYTES / 16 / kManyThreads;                /* pieces per thread          */
+    constexpr int RP = D * A::ES >= 256 ? 1 : 256 / (D * A::ES);    /* key rows per 256 bytes     */
+    static_assert(VC == 8, "a row of values is 128 bytes");
+    __shared__ __align__(16) uint8_t lds[2][2][L::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
+    const AttnHdr &h = header(a);
+    const int n_item = h.n_work[kAttnMany] * a.kv_heads;
+    const AttnWork *work = (const AttnWork *)(a.blob + h.work[kAttnMany]);
+    const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
+    for (int item = blockIdx.x; item < n_item; item += gridDim.x) {
+        const AttnWork w = work[item / a.kv_heads];
+        const int kvh = item % a.kv_heads;
+        const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
+        const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
+        AttQ<TYPE, D> q[NT];
+        AttRow<D> row[NT];
+        float c[NT];
+        int limit[NT], tok[NT], head[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int i = 32 * wave + 16 * n + col, r = w.row + i;
+            const bool any = i < w.rows;
+            tok[n] = any ? r / a.group : w.row / a.group;
+            head[n] = kvh * a.group + r % a.group;
+            limit[n] = any ? min(toks[tok[n]].pos + 1, w.key1) : 0;
+            c[n] = load_q<TYPE, D>(a.q + ((size_t)tok[n] * a.heads + head[n]) * D, any, g, a.scale_log2, q[n]);
+            row[n].ref = kLowest;
+            row[n].l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) row[n].o[k] = f32x4{ 0, 0, 0, 0 };
+        }
+        const int n_tile = (w.key1 - w.key0 + L::KT - 1) / L::KT, last = w.key1 - 1;
+        u32x4 pid;
+        auto pages = [&](int tile) {
+#pragma unroll
+            for (int i = 0; i < NG; i++) pid[i] = (uint32_t)__builtin_amdgcn_readfirstlane(tab[min(w.key0 + tile * L::KT + 16 * i, last) >> a.shift]);
+        };
+        auto copy = [&](int tile) {
+            const int key = w.key0 + tile * L::KT;
+            uint8_t *kd = lds[tile & 1][0], *vd = lds[tile & 1][1];
+            constexpr int RI = kManyThreads / RC;                   /* key rows of one pass       */
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int r = i * RI + tid / RC;                     /* key row, and its 16 keys   */
+                const int grp = RI >= 32 ? i * (RI / 16) + __builtin_amdgcn_readfirstlane(tid / RC / 16) : i * RI / 16;
+                int pg = (int)pid[0];
+#pragma unroll
+                for (int k = 1; k < NG; k++) pg = grp == k ? (int)pid[k] : pg;
+                const int m = TYPE == 1 ? (((r >> 3) & 3) << 2 | (r & 3)) : (r & 15);
+                const int piece = (tid % RC) ^ (m / RP);
+                const int slot = (key + r) & P1;
+                dma_to_lds<16>(page_at(a.k, pg, a.page_bytes, head_off) + (uint32_t)(slot * D + piece * A::CE) * A::ES,
+                               kd + (i * kManyThreads + wave * 64) * 16);
+            }
+            const int piece = (tid & 7) ^ ((tid >> 4) & 7);
+            int pg = (int)pid[0];
+#pragma unroll
+            for (int k = 1; k < NG; k++) pg = piece * A::CE / 16 == k ? (int)pid[k] : pg;
+            const int slot = (key + piece * A::CE) & P1;
+            const uint8_t *p = page_at(a.v, pg, a.page_bytes, head_off) + (uint32_t)(((tid >> 3) << a.shift) + slot) * A::ES;
+            const uint32_t step = (uint32_t)(32 * A::ES) << a.shift;
+#pragma unroll
+            for (int i = 0; i < NL; i++) dma_to_lds<16>(p + i * step, vd + (i * kManyThreads + wave * 64) * 16);
+        };
+        uint32_t bad = 0;
+        const bool idle = 32 * wave >= w.rows;
+        if (n_tile > 0) {
+            pages(0);
+            copy(0);
+            if (n_tile > 1) pages(1);
+        }
+        for (int tile = 0; tile < n_tile; tile++) {
+            mx_wait_barrier();
+            if (tile + 1 < n_tile) {
+                copy(tile + 1);
+                if (tile + 2 < n_tile) pages(tile + 2);
+            }
+            if (idle) continue;
+            const uint8_t *kt = lds[tile & 1][0], *vt = lds[tile & 1][1];
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                const int key = w.key0 + tile * L::KT + st * A::KS;
+                if (key >= w.key1) break;
+                const bool mask = key + A::KS > w.full;
+                f32x4 sc[NT][A::TL];
+                const uint8_t *kr = kt + (st * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
+                auto kget = [&](int t, int i) { return *(const u32x4 *)(kr + 4 * t * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16)); };
+                scores<TYPE, D, NT>(kget, q, sc);
+                const uint8_t *vr = vt + col * 128 + (((4 * st + g) ^ ((col >> 1) & 7)) * 16);
+                AttP<TYPE> p[NT];
+                const int at = key + g * A::CE;
+                if (mask) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) soften<TYPE, D, true>(c[n], limit[n] - at, sc[n], row[n], p[n]);
+                    const AttMask m = piece_mask<TYPE>(w.full - at, w.key1 - at);
+                    weigh<TYPE, D, NT>([&](int i) { return clean<TYPE>(*(const u32x4 *)(vr + 2048 * i), m, bad); }, p, row);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) soften<TYPE, D, false>(c[n], 0, sc[n], row[n], p[n]);
+                    weigh<TYPE, D, NT>([&](int i) { return *(const u32x4 *)(vr + 2048 * i); }, p, row);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float l = row_sum(row[n].l);
+            if (32 * wave + 16 * n + col >= w.rows) continue;
+            const AttnTok tk = toks[tok[n]];
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+                put_row(a, tk, w.part, tok[n], head[n], 16 * i + 4 * g, D, row[n].ref, l, row[n].o[i], i == 0 && g == 0);
+            if (__builtin_expect(__ballot(bad) != 0, 0)) {
+                float *o = row_out(a, tk, w.part, tok[n], head[n], D);
+#pragma unroll 1
+                for (int d = 4 * g; d < D; d += 16) {
+                    const f32x4 e = wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, limit[n], d);
+                    *(f32x4 *)(o + d) += e;
+                }
+            }
+        }
+        __syncthreads();                                            /* the buffers, before the next item */
+    }
+}
+
+/* Parts of a row joined in slot order: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. */
+template <int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
+{
+    constexpr int TPR = D / 4, RPB = 256 / TPR;
+    const AttnHdr &h = header(a);
+    const int n = h.n_comb * a.heads;
+    const int32_t *comb = (const int32_t *)(a.blob + h.comb);
+    const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
+    for (int i = blockIdx.x * RPB + threadIdx.x / TPR; i < n; i += gridDim.x * RPB) {
+        const int t = comb[i / a.heads], head = i % a.heads, d = threadIdx.x % TPR * 4;
+        const AttnTok tk = toks[t];
+        const size_t r0 = (size_t)tk.part * a.heads + head;
+        float m = kLowest;
+        for (int p = 0; p < tk.parts; p++) m = fmaxf(m, a.part_ml[2 * (r0 + (size_t)p * a.heads)]);
+        float l = 0.0f;
+        f32x4 o = { 0, 0, 0, 0 };
+        for (int p = 0; p < tk.parts; p++) {
+            const size_t r = r0 + (size_t)p * a.heads;
+            const float mp = a.part_ml[2 * r];
+            if (mp == kLowest) continue;                            /* saw no key */
+            const float f = exp2_fast(mp - m);
+            l += f * a.part_ml[2 * r + 1];
+            o += *(const f32x4 *)(a.part_o + r * D + d) * f;
+        }
+        *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + d) = o * (1.0f / l);
+    }
+}
+
+/* Head norms, rotation and the append. Units of 16 (D 128) or 32 (D 64) heads of one token: D / 8 lanes a
+ * head, each with four elements and their four partners half a head away, so that the norm's sum and
+ * the rotation stay in the lanes. Values go through LDS in tiles of up to 32 tokens of one page, so that
+ * their transposed rows are stored in runs. */
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void attn_append_kernel(AttnAppend b)
+{
+    constexpr int LPH = D / 8, HPB = 256 / LPH;
+    constexpr int ES = Att<TYPE, D>::ES;
+    __shared__ float s_v[kVTile][D + 1];
+    const AttnCall &a = b.c;
+    const AttnHdr &h = header(a);
+    const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
+    const int n_head = (b.q ? a.heads : 0) + a.kv_heads, passes = (n_head + HPB - 1) / HPB;
+    const int n_qk = h.n_tok * passes, n_unit = n_qk + h.n_vt * a.kv_heads;
+    const int P1 = (1 << a.shift) - 1;
+    for (int u = blockIdx.x; u < n_unit; u += gridDim.x) {
+        if (u < n_qk) {
+            const int t = u / passes, hd = u % passes * HPB + threadIdx.x / LPH, i0 = threadIdx.x % LPH * 4;
+            if (hd >= n_head) continue;
+            const AttnTok tk = toks[t];
+            const bool is_k = hd >= n_head - a.kv_heads;
+            const int kvh = hd - (n_head - a.kv_heads);
+            const float *x = is_k ? b.k + ((size_t)t * a.kv_heads + kvh) * D : b.q + ((size_t)t * a.heads + hd) * D;
+            f32x4 lo = *(const f32x4 *)(x + i0), hi = *(const f32x4 *)(x + D / 2 + i0);
+            if (b.norm) {
+                const float *wt = is_k ? b.kw : b.qw;
+                float ss = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) ss = __builtin_fmaf(lo[e], lo[e], __builtin_fmaf(hi[e], hi[e], ss));
+#pragma unroll
+                for (int o = 1; o < LPH; o *= 2) ss += __shfl_xor(ss, o);
+                const float inv = 1.0f / sqrtf(ss / D + b.eps);
+                lo *= inv;
+                hi *= inv;
+                if (wt) {
+                    lo *= *(const f32x4 *)(wt + i0);
+                    hi *= *(const f32x4 *)(wt + D / 2 + i0);
+                }
+            }
+            f32x4 y0, y1;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                /* the angle in turns, in double: far positions keep their fraction of a turn */
+                const double turns = (double)tk.pos * b.freq[i0 + e];
+                float sn, cs;
+                sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+                y0[e] = lo[e] * cs - hi[e] * sn;
+                y1[e] = hi[e] * cs + lo[e] * sn;
+            }
+            if (!is_k) {
+                float *y = b.qr + ((size_t)t * a.heads + hd) * D;
+                *(f32x4 *)(y + i0) = y0;
+                *(f32x4 *)(y + D / 2 + i0) = y1;
+            } else {
+                uint8_t *y = const_cast<uint8_t *>(page_at(a.k, tk.dst >> a.shift, a.page_bytes, (uint32_t)kvh * ((uint32_t)(D * ES) << a.shift))) +
+                             (uint32_t)((tk.dst & P1) * D + i0) * ES;
+                if constexpr (TYPE == 0) {
+                    *(f32x4 *)y = y0;
+                    *(f32x4 *)(y + D / 2 * ES) = y1;
+                } else {
+                    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                    *(h4 *)y = __builtin_convertvector(y0, h4);
+                    *(h4 *)(y + D / 2 * ES) = __builtin_convertvector(y1, h4);
+                }
+            }
+        } else {
+            const int kvh = (u - n_qk) % a.kv_heads;
+            const AttnVTile vt = ((const AttnVTile *)(a.blob + h.vt))[(u - n_qk) / a.kv_heads];
+            uint8_t *y = const_cast<uint8_t *>(page_at(a.v, vt.page, a.page_bytes, (uint32_t)kvh * ((uint32_t)(D * ES) << a.shift)));
+            auto put = [&](int d, int slot, float v) {
+                const uint32_t off = ((uint32_t)d << a.shift) + (uint32_t)slot;
+                if constexpr (TYPE == 0) *(float *)(y + off * ES) = v;
+                else *(_Float16 *)(y + off * ES) = (_Float16)v;
+            };
+            const float *x = b.v + ((size_t)vt.tok * a.kv_heads + kvh) * D;
+            if (vt.n == 1) {
+                if (threadIdx.x < D) put(threadIdx.x, vt.slot, x[threadIdx.x]);
+                continue;
+            }
+            for (int e = threadIdx.x; e < vt.n * (D / 4); e += 256) {
+                const f32x4 v = *(const f32x4 *)(x + (size_t)(e / (D / 4)) * a.kv_heads * D + e % (D / 4) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) s_v[e / (D / 4)][e % (D / 4) * 4 + j] = v[j];
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < kVTile * D; e += 256)
+                if (e % kVTile < vt.n) put(e / kVTile, vt.slot + e % kVTile, s_v[e % kVTile][e / kVTile]);
+            __syncthreads();
+        }
+    }
+}
+
+template <int TYPE, int D>
+hipError_t attend(const AttnCall &a, int grid, hipStream_t st)
+{
+    const int nb[kAttnKinds] = { a.live ? grid : a.h.n_work[0] * a.kv_heads, a.live ? grid : a.h.n_work[1] * a.kv_heads };
+    if (nb[kAttnMany]) QLAUNCH("attend", (attn_many_kernel<TYPE, D>), dim3((unsigned)nb[kAttnMany]), dim3(kManyThreads), 0, st, a);
+    if (nb[kAttnFew]) QLAUNCH("attend", (attn_few_kernel<TYPE, D>), dim3((unsigned)nb[kAttnFew]), dim3(64 * kFewWaves), 0, st, a);
+    const int rpb = 256 / (D / 4), nj = a.live ? grid : (a.h.n_comb * a.heads + rpb - 1) / rpb;
+    if (nj) QLAUNCH("join", (attn_join_kernel<D>), dim3((unsigned)nj), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attend(const AttnCall &a, int type, int D, int grid, hipStream_t st)
+{
+    if (type == 1) return D == 128 ? attend<1, 128>(a, grid, st) : attend<1, 64>(a, grid, st);
+    return D == 128 ? attend<0, 128>(a, grid, st) : attend<0, 64>(a, grid, st);
+}
+
+hipError_t launch_attn_append(const AttnAppend &b, int type, int D, int grid, hipStream_t st)
+{
+    const int hpb = 256 / (D / 8), n_head = (b.q ? b.c.heads : 0) + b.c.kv_heads;
+    const int units = b.c.h.n_tok * ((n_head + hpb - 1) / hpb) + b.c.h.n_vt * b.c.kv_heads;
+    const dim3 nb((unsigned)(b.c.live ? grid : units));
+    if (type == 1 && D == 128) QLAUNCH("append", (attn_append_kernel<1, 128>), nb, dim3(256), 0, st, b);
+    else if (type == 1) QLAUNCH("append", (attn_append_kernel<1, 64>), nb, dim3(256), 0, st, b);
+    else if (D == 128) QLAUNCH("append", (attn_append_kernel<0, 128>), nb, dim3(256), 0, st, b);
+    else QLAUNCH("append", (attn_append_kernel<0, 64>), nb, dim3(256), 0, st, b);
+    return hipGetLastError();
+}
+
+}  // namespace qmsg

@@ -40,6 +40,22 @@ __device__ __forceinline__ void mx_lds_barrier()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+/* The LDS DMA: `bytes` (4 or 16) from src of every active lane to dst + lane * bytes. */
+template <int BYTES>
+__device__ __forceinline__ void dma_to_lds(const void *src, uint8_t *dst)
+{
+    if constexpr (BYTES == 4) __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void *)dst, 4, 0, 0);
+    else __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+
+/* Wait for all of this wave's vector memory instructions (its LDS DMA included) and LDS
+ * accesses, then the block barrier. The memory clobber keeps the compiler from moving LDS
+ * accesses across it. */
+__device__ __forceinline__ void mx_wait_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 }  // namespace qmsg
 
 #endif /* QMSG_DEVICE_H */

@@ -2992,22 +2992,6 @@ __device__ __forceinline__ void mx_chunk16_q6(const uint8_t *W, uint32_t off, co
     mx_block16_q6<NQ, O, 7, NT, TS>(st, acc, cr);
 }
 
-/* The LDS DMA: `bytes` (4 or 16) from src of every active lane to dst + lane * bytes. */
-template <int BYTES>
-__device__ __forceinline__ void dma_to_lds(const void *src, uint8_t *dst)
-{
-    if constexpr (BYTES == 4) __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void *)dst, 4, 0, 0);
-    else __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
-}
-
-/* Wait for all of this wave's vector memory instructions (its LDS DMA included) and LDS
- * accesses, then the block barrier. The memory clobber keeps the compiler from moving LDS
- * accesses across it. */
-__device__ __forceinline__ void mx_wait_barrier()
-{
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 /* Waves per SIMD the MFMA kernel is built for: six where three double-buffered blocks' LDS
  * fits a CU, else four (the register budget follows: 80 or 128 VGPRs). */
 template <int TYPE, int WSG, int PPW, int NW, int NB, int NT>

@@ -1,0 +1,84 @@
+/* qmsg_plan.h - a batch of sequences laid out as work for the attention kernels. Host code without
+ * the HIP runtime: qmsg_attn_batch checks a batch and plans it here, the kernels read the result.
+ *
+ * Rows are (token, query head of the kv head's group), token-major: row t * G + g. A work item is a
+ * tile of rows against a range of keys of one page table, for every kv head. Rows whose keys are
+ * spread over several items leave partial results (reference maximum, sum, weighted values) in
+ * slots of their own, which the combine kernel joins in slot order. */
+#ifndef QMSG_PLAN_H
+#define QMSG_PLAN_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <string>
+#include <vector>
+
+namespace qmsg {
+
+/* A token of the batch. */
+struct AttnTok {
+    int32_t pos;      /* position in its sequence: it sees keys 0 .. pos */
+    int32_t dst;      /* page * page_tokens + slot of its key and value   */
+    int32_t part;     /* first partial slot, where parts > 1              */
+    int32_t parts;    /* items its keys are spread over                   */
+};
+
+/* Up to kVTile tokens whose values go to neighbouring slots of one page. */
+struct AttnVTile {
+    int32_t tok, n, page, slot;
+};
+constexpr int kVTile = 32;
+
+struct AttnWork {
+    int32_t row, rows;      /* first row and rows of the tile                             */
+    int32_t pages;          /* the page table, as an index into the batch's page ids     */
+    int32_t key0, key1;     /* keys of this item (key0 a multiple of 16)                  */
+    int32_t full;           /* every row sees the keys below this one                     */
+    int32_t part;           /* which of its rows' partial slots it fills                  */
+    int32_t pad;
+};
+
+/* Row tiles of the kernels: waves that split the keys, waves that split the rows and share the keys
+ * through LDS. */
+enum { kAttnFew = 0, kAttnMany = 1, kAttnKinds = 2 };
+constexpr int kAttnRows[kAttnKinds] = { 16, 128 };
+/* A segment's keys are spread over at most this many items. */
+constexpr int kAttnSplits = 64;
+
+/* Where the parts of a batch sit in its blob (byte offsets) and how many there are. */
+struct AttnHdr {
+    int32_t n_tok, n_vt, n_comb, n_work[kAttnKinds];
+    int32_t tok, vt, comb, work[kAttnKinds], pages, bytes;
+};
+
+struct AttnShape {
+    int heads, kv_heads, D, type, page, n_page;
+    int max_seq, max_tokens, max_pages;
+};
+
+/* Partial rows (one query head of one token and slot) of a context's workspace. */
+constexpr size_t kAttnPartRows = (size_t)1 << 18;
+inline size_t attn_part_rows(const AttnShape &s)
+{
+    const size_t most = (size_t)s.max_tokens * (size_t)s.heads * 2 * kAttnSplits;
+    return most < kAttnPartRows ? most : kAttnPartRows;
+}
+/* Bytes that hold any batch of this shape. */
+size_t attn_blob_bytes(const AttnShape &s);
+
+struct AttnPlan {
+    AttnHdr h{};
+    std::vector<uint8_t> blob;            /* header, then the parts */
+    std::vector<int64_t> owner;           /* per page: the last batch that writes it */
+    int64_t batches = 0;
+};
+
+/* Plan n_seq sequences: q_len[i] new tokens, the last of kv_len[i] tokens, on pages
+ * [i * stride ..]. Returns an empty string, or what is wrong with the batch (p keeps its last). */
+std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len, const int *kv_len, const int32_t *pages,
+                      int stride, AttnPlan *p);
+
+}  // namespace qmsg
+
+#endif /* QMSG_PLAN_H */

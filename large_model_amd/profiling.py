@@ -33,6 +33,7 @@ SHORT = {
     "copy_kernel": "copy", "dense_kernel": "dense", "dense_oct_kernel": "dense", "dense_tok_kernel": "dense",
     "dense_any_kernel": "dense", "chain_dense_kernel": "dense", "dense_quant_kernel": "dquant",
     "dense_mx_quant_kernel": "dquant", "rmsnorm_kernel": "rmsnorm", "add_rows_kernel": "add",
+    "attn_append_kernel": "append", "attn_few_kernel": "attend", "attn_many_kernel": "attend", "attn_join_kernel": "join",
 }
 
 

@@ -70,6 +70,12 @@ class _Tensor(ctypes.Structure):
                 ("nbytes", ctypes.c_uint64)]
 
 
+class _AttnCfg(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in
+                ("n_head", "n_head_kv", "head_dim", "type", "page_tokens", "n_page", "n_layer", "max_seq", "max_tokens",
+                 "max_pages", "qk_norm")] + [("rope_base", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
 class _Debug(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in
                 ("logits", "sel", "wt", "start", "slot_t", "slot_of", "active", "n_active", "xq", "gu", "act",
@@ -123,6 +129,13 @@ _SIGS = {
                             ctypes.POINTER(_I)]),
     "qmsg_matmul_n": (_I, [_P, _P, _I, _P, _I, _P]),
     "qmsg_matmul_n_device": (_I, [_P, _P, _I, _P, _I, _P]),
+    "qmsg_attn_cache_bytes": (ctypes.c_uint64, [ctypes.POINTER(_AttnCfg)]),
+    "qmsg_attn_create": (_I, [_P, ctypes.POINTER(_AttnCfg), _P, _P, ctypes.POINTER(_I)]),
+    "qmsg_attn_cache": (_I, [_P, _I, ctypes.POINTER(_P), ctypes.POINTER(_P)]),
+    "qmsg_attn_norms": (_I, [_P, _I, _I, _P, _P]),
+    "qmsg_attn_batch": (_I, [_P, _I, _I, _P, _P, _P, _I]),
+    "qmsg_attn_append_device": (_I, [_P, _I, _I, _P, _P, _P, _P, ctypes.c_float]),
+    "qmsg_attn_device": (_I, [_P, _I, _I, _P, _P]),
     "qmsg_device_info": (_I, [_P, ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(ctypes.c_uint64),
                               ctypes.c_char_p, _I]),
 }
@@ -411,6 +424,51 @@ class Context:
         self._check(lib.qmsg_block_dots(self._h, layer, which, expert.shape[0], _ptr(expert), _ptr(row),
                                         _ptr(block), _ptr(xq_blocks), _ptr(out)))
         return out
+
+    # ---------------------------------------------------------------- attention
+    def attn_create(self, n_head: int, n_head_kv: int, head_dim: int, type_: int = QMSG_T_F16, page: int = 64,
+                    n_page: int = 1, n_layer: int = 1, rope_base: float = 1e6, qk_norm: bool = True, scale: float = 0.0,
+                    max_seq: int = 1, max_tokens: int = 1, max_pages: int = 1, d_k: Optional[int] = None,
+                    d_v: Optional[int] = None) -> int:
+        """An attention over a paged cache (the context's, or the caller's d_k and d_v); returns its id."""
+        cfg = _AttnCfg(n_head, n_head_kv, head_dim, type_, page, n_page, n_layer, max_seq, max_tokens, max_pages,
+                       int(qk_norm), rope_base, scale)
+        i = _I()
+        self._check(lib.qmsg_attn_create(self._h, ctypes.byref(cfg), d_k, d_v, ctypes.byref(i)))
+        self._attns = getattr(self, "_attns", {})
+        self._attns[i.value] = cfg
+        return i.value
+
+    def attn_cache(self, attn: int) -> tuple:
+        """Device addresses of the keys [layer][page][kv head][slot][D] and the values [layer][page][kv head][D][slot]."""
+        k, v = _P(), _P()
+        self._check(lib.qmsg_attn_cache(self._h, attn, ctypes.byref(k), ctypes.byref(v)))
+        return k.value, v.value
+
+    def attn_norms(self, attn: int, layer: int, q_norm: Optional[np.ndarray], k_norm: Optional[np.ndarray]):
+        """A layer's head norm weights (None: unit weights)."""
+        w = [None if a is None else np.ascontiguousarray(a, np.float32) for a in (q_norm, k_norm)]
+        d = self._attns[attn].head_dim if attn in getattr(self, "_attns", {}) else None
+        if d is not None and any(a is not None and a.size != d for a in w):
+            raise ValueError(f"head norms have {d} weights")
+        self._check(lib.qmsg_attn_norms(self._h, attn, layer, _ptr(w[0]), _ptr(w[1])))
+
+    def attn_batch(self, attn: int, q_len, kv_len, pages):
+        """The sequences of the next calls: q_len[i] new of kv_len[i] tokens on pages[i] (int32 [n][pages])."""
+        q, kv = np.ascontiguousarray(q_len, np.int32), np.ascontiguousarray(kv_len, np.int32)
+        pages = np.ascontiguousarray(pages, np.int32)
+        if pages.ndim != 2 or q.shape != (len(pages),) or kv.shape != q.shape:
+            raise ValueError("q_len and kv_len have an entry, pages a row, for each sequence")
+        self._check(lib.qmsg_attn_batch(self._h, attn, len(q), _ptr(q), _ptr(kv), _ptr(pages), pages.shape[1]))
+
+    def attn_append_device(self, attn: int, layer: int, d_qr: Optional[int], d_q: Optional[int], d_k: int, d_v: int,
+                           eps: float = 1e-6):
+        """Norm and rotate the batch's query heads into d_qr and write its keys and values into the cache."""
+        self._check(lib.qmsg_attn_append_device(self._h, attn, layer, d_qr, d_q, d_k, d_v, eps))
+
+    def attn_device(self, attn: int, layer: int, d_q: int, d_out: int):
+        """d_out = the batch's attention over the cache, each token seeing its sequence up to its own position."""
+        self._check(lib.qmsg_attn_device(self._h, attn, layer, d_q, d_out))
 
     # ---------------------------------------------------------------- device buffers / timing
     def device_alloc(self, nbytes: int) -> int:

@@ -1,0 +1,208 @@
+"""Attention over the paged cache on the GPU against float64: head layouts, lengths, pages, masks, shared prefixes."""
+import numpy as np
+import pytest
+
+from attn_cases import EPS32, F16, F32, Batch, attend64, dtype_of, pack, values
+
+pytestmark = pytest.mark.gpu
+
+TINY = (256, 16, 4, 128)
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from large_model_amd import qmsg
+    with qmsg.Context(*TINY, n_layer=1, max_tokens=1) as c:
+        yield c
+
+
+class Pool:
+    """An attention and its pools in the context, device rows for a batch."""
+
+    def __init__(self, ctx, heads, kv_heads, D, type_, batch, n_layer=1, **kw):
+        self.ctx, self.H, self.D, self.b = ctx, heads, D, batch
+        self.id = ctx.attn_create(heads, kv_heads, D, type_=type_, page=batch.page, n_page=batch.n_page, n_layer=n_layer,
+                                  max_seq=max(1, len(batch.q)), max_tokens=max(1, batch.T), max_pages=batch.max_pages, **kw)
+        self.k, self.v = ctx.attn_cache(self.id)
+
+    def run(self, q, kp, vp, layer=0):
+        """out [T][H][D] with rows of a canary behind it, which have to stay."""
+        ctx, b = self.ctx, self.b
+        ctx.h2d(self.k + layer * kp.nbytes, kp)
+        ctx.h2d(self.v + layer * vp.nbytes, vp)
+        d_q, d_o = ctx.device_alloc(q.nbytes + 16), ctx.device_alloc(q.nbytes + 4096)
+        ctx.h2d(d_q, q)
+        ctx.h2d(d_o, np.full(q.size + 1024, 7.0, np.float32))
+        ctx.attn_batch(self.id, b.q, b.kv, b.pages)
+        ctx.attn_device(self.id, layer, d_q, d_o)
+        ctx.sync()
+        o = ctx.d2h(d_o, q.size + 1024)
+        assert np.all(o[q.size:] == 7.0), "rows behind the batch were written"
+        return o[:q.size].reshape(q.shape)
+
+
+def check(got, want, tol):
+    assert np.array_equal(np.isnan(got), np.isnan(want)) or np.all(np.isfinite(got)), "not finite"
+    off = np.abs(got - want)
+    i = np.unravel_index(np.argmax(off - tol), off.shape)
+    assert np.all(off <= tol), f"at {i}: {got[i]} for {want[i]}, {off[i]:.3g} off, {tol[i]:.3g} allowed"
+
+
+HEADS = [(14, 2, 64), (16, 16, 128), (32, 4, 128), (64, 4, 128), (6, 2, 64), (8, 8, 64), (64, 1, 128)]
+LENS = {
+    "one": [(1, 1)],
+    "ends": [(1, 15), (1, 16), (1, 17), (1, 31), (1, 32), (1, 33), (1, 63), (1, 64), (1, 65)],
+    "ragged": [(1, 300), (0, 40), (1, 1), (1, 777), (0, 0), (1, 129)],
+    "draft": [(5, 5), (3, 260), (8, 515)],
+    "prompt": [(33, 33), (130, 130), (1, 90), (65, 301)],
+}
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads", HEADS, ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("lens", list(LENS))
+def test_attention(ctx, lens, heads, type_):
+    H, kv, D = heads
+    page = {"one": 16, "ends": 16, "ragged": 64, "draft": 32, "prompt": 128}[lens]
+    print(f"[case] {lens} {heads} type {type_}", flush=True)
+    b = Batch(LENS[lens], page, seed=H + D)
+    k, v = values(b, kv, D, type_, 1)
+    q = (2 * np.random.default_rng(2).standard_normal((b.T, H, D))).astype(np.float32)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))      # NaN in every other slot
+    check(got, *attend64(b, q, k, v, D ** -0.5))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("type_", [F16, F32])
+def test_every_key_counts_once(ctx, page, type_):
+    """Equal scores and whole values: sums are exact, so that one key more or less shows."""
+    b = Batch([(1, 1000), (40, 777), (1, 5), (3, 3), (1, 2049), (7, 391)], page, seed=page)
+    kv, D, H = 2, 128, 16
+    k, v = values(b, kv, D, type_, 3)
+    v = [np.round(a * 3).astype(dtype_of(type_)) for a in v]
+    q = np.zeros((b.T, H, D), np.float32)
+    print(f"[case] equal scores, pages of {page}, type {type_}", flush=True)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    want = np.stack([np.repeat(v[s][:p + 1].astype(np.float64).mean(0), H // kv, 0) for s, p in zip(b.seq, b.pos)])
+    assert np.all(np.abs(got - want) <= 4 * EPS32 * np.abs(want))          # the reciprocal, its product, the output
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("what", ["one", "two_runs", "tokens", "wide", "idle"])
+def test_shared_prefix(ctx, what, type_):
+    H, kv, D, page = 32, 4, 128, 32
+    shared, runs, lens = {
+        "one": (512, None, [(1, 513), (1, 700), (1, 900), (1, 530)]),
+        "two_runs": (320, [3, 1, 2], [(1, 321), (1, 480), (1, 322), (1, 333), (1, 600), (1, 345)]),
+        "tokens": (288, None, [(3, 300), (1, 289), (2, 290), (6, 400)]),
+        "wide": (1024, None, [(1, 1025 + 37 * i) for i in range(24)]),
+        "idle": (256, None, [(1, 300), (0, 300), (1, 512), (2, 301)]),
+    }[what]
+    print(f"[case] shared prefix {what} type {type_}", flush=True)
+    b = Batch(lens, page, shared, runs, seed=5)
+    k, v = values(b, kv, D, type_, 4, shared, runs)
+    q = (2 * np.random.default_rng(6).standard_normal((b.T, H, D))).astype(np.float32)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    check(got, *attend64(b, q, k, v, D ** -0.5))
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("n", [6, 150])
+def test_what_a_row_does_not_see(ctx, type_, bad, n):
+    """Infinities and NaN in later tokens' keys and values do not reach earlier rows; those that see them get them."""
+    H, kv, D = 8, 2, 64
+    b = Batch([(n, 200), (1, 77)], 16, seed=8)
+    k, v = values(b, kv, D, type_, 9)
+    p_v, p_k = 200 - n + n // 3, 200 - n + 2 * n // 3
+    v[0][p_v, 1, 5] = bad
+    k[0][p_k, 0, 3] = np.nan
+    print(f"[case] {bad} from position {p_v}, type {type_}, {n} rows", flush=True)
+    q = np.random.default_rng(10).standard_normal((b.T, H, D)).astype(np.float32)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    want, tol = attend64(b, q, k, v, D ** -0.5)
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), fine)
+    assert not fine[:n, 4:, 5][p_v - 200 + n:].any() and not fine[:n, :4][p_k - 200 + n:].any() and fine[n:].all()
+    check(got[fine], want[fine], tol[fine])
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+def test_score_and_query_ranges(ctx, type_):
+    """Scores of thousands, rows of zeros, of tiny and of large queries."""
+    H, kv, D = 16, 2, 64
+    b = Batch([(1, 700), (20, 333)], 64, seed=11)
+    k, v = values(b, kv, D, type_, 12)
+    q = np.random.default_rng(13).standard_normal((b.T, H, D)).astype(np.float32)
+    q[0, 0] *= 3000
+    q[0, 1] = 0
+    q[1, 2] *= 1e-30
+    q[2, 3] *= 1e-42                       # subnormal
+    q[3, 4] *= 500
+    q[4] *= np.float32(2.0) ** np.arange(-20, 12, 2)[:, None].astype(np.float32)
+    print(f"[case] ranges, type {type_}", flush=True)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    check(got, *attend64(b, q, k, v, D ** -0.5))
+
+
+def test_scale_and_layers(ctx):
+    H, kv, D = 8, 2, 128
+    b = Batch([(1, 100), (4, 60)], 32, seed=14)
+    q = np.random.default_rng(15).standard_normal((b.T, H, D)).astype(np.float32)
+    pool = Pool(ctx, H, kv, D, F16, b, n_layer=3, scale=0.25)
+    print("[case] scale, layers", flush=True)
+    for layer in (2, 0, 1):
+        k, v = values(b, kv, D, F16, 20 + layer)
+        check(pool.run(q, *pack(b, k, v, kv, D, F16), layer=layer), *attend64(b, q, k, v, 0.25))
+
+
+def test_offsets_past_32_bits(ctx):
+    """Pages that start beyond 2^32 bytes and 2^31 elements of a pool."""
+    H, kv, D, page, n_page = 16, 16, 128, 256, 4300
+    b = Batch([(1, 700), (3, 515)], page, seed=16)
+    b.pages = np.where(b.pages >= 0, b.pages + n_page - b.n_page, b.pages).astype(np.int32)
+    k, v = values(b, kv, D, F32, 17)
+    q = np.random.default_rng(18).standard_normal((b.T, H, D)).astype(np.float32)
+    shift = n_page - b.n_page
+    print("[case] far pages", flush=True)
+    from large_model_amd import qmsg
+    with qmsg.Context(*TINY, n_layer=1, max_tokens=1) as c:      # the pools go with it
+        small = b.n_page
+        b.n_page = n_page
+        pool = Pool(c, H, kv, D, F32, b)
+        b.n_page, b.pages = small, b.pages - shift
+        kp, vp = pack(b, k, v, kv, D, F32)
+        b.pages = b.pages + shift
+        off = shift * kv * page * D * 4
+        assert off > 2 ** 33
+        pool.k, pool.v = pool.k + off, pool.v + off
+        check(pool.run(q, kp, vp), *attend64(b, q, k, v, D ** -0.5))
+
+
+def test_empty_batches(ctx):
+    b = Batch([(0, 5), (0, 0)], 16, seed=19)
+    pool = Pool(ctx, 8, 2, 64, F16, b)
+    d = ctx.device_alloc(4096)
+    print("[case] no new tokens", flush=True)
+    ctx.h2d(d, np.full(1024, 3.0, np.float32))
+    ctx.attn_device(pool.id, 0, d, d + 2048)                     # before any batch
+    ctx.attn_batch(pool.id, b.q, b.kv, b.pages)
+    ctx.attn_device(pool.id, 0, d, d + 2048)
+    ctx.attn_append_device(pool.id, 0, d, d, d + 1024, d + 2048)
+    ctx.attn_batch(pool.id, [], [], np.zeros((0, 1), np.int32))
+    ctx.attn_device(pool.id, 0, d, d + 2048)
+    ctx.sync()
+    assert np.all(ctx.d2h(d, 1024) == 3.0)
+
+
+def test_same_call_same_bits(ctx):
+    H, kv, D = 64, 4, 128
+    b = Batch([(1, 3000), (5, 900), (100, 100)], 64, seed=21)
+    k, v = values(b, kv, D, F16, 22)
+    q = np.random.default_rng(23).standard_normal((b.T, H, D)).astype(np.float32)
+    kp, vp = pack(b, k, v, kv, D, F16)
+    pool = Pool(ctx, H, kv, D, F16, b)
+    print("[case] the same call again", flush=True)
+    first = pool.run(q, kp, vp)
+    for _ in range(3):
+        assert np.array_equal(pool.run(q, kp, vp), first)
