@@ -22,6 +22,7 @@
  * largest score so far and raised only when a score passes it by 14, so that p stays below 2^14 (f16's
  * range) and the usual step needs no reduction across lanes. Sums, references and O are fp32. */
 #include <cmath>
+#include <type_traits>
 
 #include "qmsg_attn.h"
 #include "qmsg_device.h"
@@ -466,7 +467,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 /* Many rows (128): four waves of 32 rows each share tiles of keys and values, copied to LDS by the LDS
  * DMA, the next tile's copy in flight while one is worked on. Pieces are stored with their index in
  * the row xored by the row, so that the 16 rows a wave instruction reads lie in all banks. */
-constexpr int kManyThreads = 256;
+constexpr int kManyNT = 1;
+constexpr int kManyThreads = 64 * 128 / (16 * kManyNT);
 
 template <int TYPE, int D>
 struct ManyLds {
@@ -475,11 +477,11 @@ struct ManyLds {
 };
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
+__global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_kernel(AttnCall a)
 {
     using A = Att<TYPE, D>;
     using L = ManyLds<TYPE, D>;
-    constexpr int NT = 2, RC = D / A::CE, VC = L::KT / A::CE, NG = L::KT / 16;
+    constexpr int NT = kManyNT, RC = D / A::CE, VC = L::KT / A::CE, NG = L::KT / 16;
     constexpr int NL = L::BYTES / 16 / kManyThreads;                /* pieces per thread          */
     constexpr int RP = D * A::ES >= 256 ? 1 : 256 / (D * A::ES);    /* key rows per 256 bytes     */
     static_assert(VC == 8, "a row of values is 128 bytes");
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
         int limit[NT], tok[NT], head[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int i = 32 * wave + 16 * n + col, r = w.row + i;
+            const int i = 16 * NT * wave + 16 * n + col, r = w.row + i;
             const bool any = i < w.rows;
             tok[n] = any ? r / a.group : w.row / a.group;
             head[n] = kvh * a.group + r % a.group;
@@ -525,7 +527,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int r = i * RI + tid / RC;                     /* key row, and its 16 keys   */
-                const int grp = RI >= 32 ? i * (RI / 16) + __builtin_amdgcn_readfirstlane(tid / RC / 16) : i * RI / 16;
+                const int grp = __builtin_amdgcn_readfirstlane(r / 16);
                 int pg = (int)pid[0];
 #pragma unroll
                 for (int k = 1; k < NG; k++) pg = grp == k ? (int)pid[k] : pg;
@@ -541,53 +543,60 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
             for (int k = 1; k < NG; k++) pg = piece * A::CE / 16 == k ? (int)pid[k] : pg;
             const int slot = (key + piece * A::CE) & P1;
             const uint8_t *p = page_at(a.v, pg, a.page_bytes, head_off) + (uint32_t)(((tid >> 3) << a.shift) + slot) * A::ES;
-            const uint32_t step = (uint32_t)(32 * A::ES) << a.shift;
+            const uint32_t step = (uint32_t)(kManyThreads / 8 * A::ES) << a.shift;
 #pragma unroll
             for (int i = 0; i < NL; i++) dma_to_lds<16>(p + i * step, vd + (i * kManyThreads + wave * 64) * 16);
         };
         uint32_t bad = 0;
-        const bool idle = 32 * wave >= w.rows;
+        const bool idle = 16 * NT * wave >= w.rows;
         if (n_tile > 0) {
             pages(0);
             copy(0);
             if (n_tile > 1) pages(1);
         }
-        for (int tile = 0; tile < n_tile; tile++) {
+        auto turn = [&](int tile) {                                 /* tile's copy is there, the next one starts */
             mx_wait_barrier();
             if (tile + 1 < n_tile) {
                 copy(tile + 1);
                 if (tile + 2 < n_tile) pages(tile + 2);
             }
-            if (idle) continue;
-            const uint8_t *kt = lds[tile & 1][0], *vt = lds[tile & 1][1];
+        };
+        auto step = [&](auto masked, int tile, int st) {
+            constexpr bool MASK = decltype(masked)::value;
+            const uint8_t *kr = lds[tile & 1][0] + (st * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
+            const uint8_t *vr = lds[tile & 1][1] + col * 128 + (((4 * st + g) ^ ((col >> 1) & 7)) * 16);
+            f32x4 sc[NT][A::TL];
+            scores<TYPE, D, NT>([&](int t, int i) { return *(const u32x4 *)(kr + 4 * t * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16)); }, q, sc);
+            AttP<TYPE> p[NT];
+            const int at = w.key0 + tile * L::KT + st * A::KS + g * A::CE;
 #pragma unroll
-            for (int st = 0; st < 2; st++) {
-                const int key = w.key0 + tile * L::KT + st * A::KS;
-                if (key >= w.key1) break;
-                const bool mask = key + A::KS > w.full;
-                f32x4 sc[NT][A::TL];
-                const uint8_t *kr = kt + (st * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
-                auto kget = [&](int t, int i) { return *(const u32x4 *)(kr + 4 * t * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16)); };
-                scores<TYPE, D, NT>(kget, q, sc);
-                const uint8_t *vr = vt + col * 128 + (((4 * st + g) ^ ((col >> 1) & 7)) * 16);
-                AttP<TYPE> p[NT];
-                const int at = key + g * A::CE;
-                if (mask) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) soften<TYPE, D, true>(c[n], limit[n] - at, sc[n], row[n], p[n]);
-                    const AttMask m = piece_mask<TYPE>(w.full - at, w.key1 - at);
-                    weigh<TYPE, D, NT>([&](int i) { return clean<TYPE>(*(const u32x4 *)(vr + 2048 * i), m, bad); }, p, row);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) soften<TYPE, D, false>(c[n], 0, sc[n], row[n], p[n]);
-                    weigh<TYPE, D, NT>([&](int i) { return *(const u32x4 *)(vr + 2048 * i); }, p, row);
-                }
+            for (int n = 0; n < NT; n++) soften<TYPE, D, MASK>(c[n], limit[n] - at, sc[n], row[n], p[n]);
+            if constexpr (MASK) {
+                const AttMask m = piece_mask<TYPE>(w.full - at, w.key1 - at);
+                weigh<TYPE, D, NT>([&](int i) { return clean<TYPE>(*(const u32x4 *)(vr + 2048 * i), m, bad); }, p, row);
+            } else {
+                weigh<TYPE, D, NT>([&](int i) { return *(const u32x4 *)(vr + 2048 * i); }, p, row);
             }
+        };
+        const int n_clear = max(0, w.full - w.key0) / L::KT;        /* tiles that every row sees whole */
+        for (int tile = 0; tile < n_clear; tile++) {
+            turn(tile);
+            if (idle) continue;
+#pragma unroll
+            for (int st = 0; st < 2; st++) step(std::false_type{}, tile, st);
+        }
+#pragma unroll 1
+        for (int tile = n_clear; tile < n_tile; tile++) {
+            turn(tile);
+            if (idle) continue;
+#pragma unroll 1
+            for (int st = 0; st < 2; st++)
+                if (w.key0 + tile * L::KT + st * A::KS < w.key1) step(std::true_type{}, tile, st);
         }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const float l = row_sum(row[n].l);
-            if (32 * wave + 16 * n + col >= w.rows) continue;
+            if (16 * NT * wave + 16 * n + col >= w.rows) continue;
             const AttnTok tk = toks[tok[n]];
 #pragma unroll
             for (int i = 0; i < D / 16; i++)
@@ -605,32 +614,53 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
     }
 }
 
-/* Parts of a row joined in slot order: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. */
-template <int D>
+/* Parts of a row joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. PL lanes of D / 4 threads take
+ * every PL-th part in slot order, then lane 0 takes the lanes' results in theirs. */
+constexpr int kJoinLanes = 8;
+
+template <int D, int PL>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
 {
-    constexpr int TPR = D / 4, RPB = 256 / TPR;
+    constexpr int TPR = D / 4, RPB = 256 / (TPR * PL);
+    __shared__ __align__(16) f32x4 s_o[PL][RPB][TPR];
+    __shared__ float s_m[PL][RPB], s_l[PL][RPB];
     const AttnHdr &h = header(a);
-    const int n = h.n_comb * a.heads;
+    const int n = h.n_comb * a.heads, d = threadIdx.x % TPR, pl = threadIdx.x / TPR % PL, rb = threadIdx.x / (TPR * PL);
     const int32_t *comb = (const int32_t *)(a.blob + h.comb);
     const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
-    for (int i = blockIdx.x * RPB + threadIdx.x / TPR; i < n; i += gridDim.x * RPB) {
-        const int t = comb[i / a.heads], head = i % a.heads, d = threadIdx.x % TPR * 4;
+    for (int i0 = blockIdx.x * RPB; i0 < n; i0 += gridDim.x * RPB) {
+        const int i = min(i0 + rb, n - 1), t = comb[i / a.heads], head = i % a.heads;
         const AttnTok tk = toks[t];
         const size_t r0 = (size_t)tk.part * a.heads + head;
-        float m = kLowest;
-        for (int p = 0; p < tk.parts; p++) m = fmaxf(m, a.part_ml[2 * (r0 + (size_t)p * a.heads)]);
-        float l = 0.0f;
+        float m = kLowest, l = 0.0f;
         f32x4 o = { 0, 0, 0, 0 };
-        for (int p = 0; p < tk.parts; p++) {
-            const size_t r = r0 + (size_t)p * a.heads;
-            const float mp = a.part_ml[2 * r];
-            if (mp == kLowest) continue;                            /* saw no key */
-            const float f = exp2_fast(mp - m);
-            l += f * a.part_ml[2 * r + 1];
-            o += *(const f32x4 *)(a.part_o + r * D + d) * f;
+        auto add = [&](float mp, float lp, f32x4 op) {
+            if (mp == kLowest) return;                              /* saw no key */
+            const float top = fmaxf(m, mp), f0 = m == kLowest ? 0.0f : exp2_fast(m - top), f1 = exp2_fast(mp - top);
+            m = top;
+            l = l * f0 + lp * f1;
+            o = o * f0 + op * f1;
+        };
+        /* two parts' loads at a time */
+        for (int p = pl; p < tk.parts; p += 2 * PL) {
+            const size_t r = r0 + (size_t)p * a.heads, r2 = p + PL < tk.parts ? r + (size_t)PL * a.heads : r;
+            const float m1 = a.part_ml[2 * r], l1 = a.part_ml[2 * r + 1], m2 = a.part_ml[2 * r2], l2 = a.part_ml[2 * r2 + 1];
+            const f32x4 o1 = *(const f32x4 *)(a.part_o + r * D + 4 * d), o2 = *(const f32x4 *)(a.part_o + r2 * D + 4 * d);
+            add(m1, l1, o1);
+            if (r2 != r) add(m2, l2, o2);
         }
-        *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + d) = o * (1.0f / l);
+        if constexpr (PL > 1) {
+            s_o[pl][rb][d] = o;
+            if (d == 0) {
+                s_m[pl][rb] = m;
+                s_l[pl][rb] = l;
+            }
+            __syncthreads();
+            if (pl == 0)
+                for (int k = 1; k < PL; k++) add(s_m[k][rb], s_l[k][rb], s_o[k][rb][d]);
+            __syncthreads();
+        }
+        if (pl == 0 && i0 + rb < n) *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + 4 * d) = o * (1.0f / l);
     }
 }
 
@@ -733,8 +763,11 @@ hipError_t attend(const AttnCall &a, int grid, hipStream_t st)
     const int nb[kAttnKinds] = { a.live ? grid : a.h.n_work[0] * a.kv_heads, a.live ? grid : a.h.n_work[1] * a.kv_heads };
     if (nb[kAttnMany]) QLAUNCH("attend", (attn_many_kernel<TYPE, D>), dim3((unsigned)nb[kAttnMany]), dim3(kManyThreads), 0, st, a);
     if (nb[kAttnFew]) QLAUNCH("attend", (attn_few_kernel<TYPE, D>), dim3((unsigned)nb[kAttnFew]), dim3(64 * kFewWaves), 0, st, a);
-    const int rpb = 256 / (D / 4), nj = a.live ? grid : (a.h.n_comb * a.heads + rpb - 1) / rpb;
-    if (nj) QLAUNCH("join", (attn_join_kernel<D>), dim3((unsigned)nj), dim3(256), 0, st, a);
+    /* rows of few parts a thread group each, others kJoinLanes groups */
+    const bool wide = a.live || a.h.max_parts > 4;
+    const int rpb = 256 / (D / 4 * (wide ? kJoinLanes : 1)), nj = a.live ? grid : (a.h.n_comb * a.heads + rpb - 1) / rpb;
+    if (nj && wide) QLAUNCH("join", (attn_join_kernel<D, kJoinLanes>), dim3((unsigned)nj), dim3(256), 0, st, a);
+    else if (nj) QLAUNCH("join", (attn_join_kernel<D, 1>), dim3((unsigned)nj), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

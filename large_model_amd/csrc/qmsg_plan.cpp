@@ -39,8 +39,20 @@ int kind_of(int rows) { return rows <= kAttnRows[kAttnFew] ? kAttnFew : kAttnMan
 int tiles_of(const Segment &g, int G) { return (g.n_tok * G + kAttnRows[g.kind] - 1) / kAttnRows[g.kind]; }
 
 /* Blocks that fill the card, and the fewest keys worth an item of their own. */
-constexpr int kBlocksPerCu[kAttnKinds] = { 4, 4 };
-constexpr int kMinKeys[kAttnKinds] = { 256, 256 };
+#ifndef FEWB
+#define FEWB 2
+#endif
+#ifndef MANYB
+#define MANYB 2
+#endif
+#ifndef FEWK
+#define FEWK 256
+#endif
+#ifndef MANYK
+#define MANYK 256
+#endif
+constexpr int kBlocksPerCu[kAttnKinds] = { FEWB, MANYB };
+constexpr int kMinKeys[kAttnKinds] = { FEWK, MANYK };
 
 /* The fewest shared keys that are read once for all. */
 constexpr int kMinShared = 256;
@@ -228,6 +240,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     h.n_tok = (int)T;
     h.n_vt = (int)vt.size();
     h.n_comb = (int)comb.size();
+    for (const AttnTok &k : tok) h.max_parts = std::max(h.max_parts, k.parts);
     h.tok = place(tok.size() * sizeof(AttnTok));
     h.vt = place(vt.size() * sizeof(AttnVTile));
     h.comb = place(comb.size() * 4);

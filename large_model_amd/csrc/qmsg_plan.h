@@ -48,7 +48,7 @@ constexpr int kAttnSplits = 64;
 
 /* Where the parts of a batch sit in its blob (byte offsets) and how many there are. */
 struct AttnHdr {
-    int32_t n_tok, n_vt, n_comb, n_work[kAttnKinds];
+    int32_t n_tok, n_vt, n_comb, max_parts, n_work[kAttnKinds];
     int32_t tok, vt, comb, work[kAttnKinds], pages, bytes;
 };
 
