@@ -57,11 +57,12 @@ struct AttQ<0, D> {
     f32x4 v[Att<0, D>::NCH];
 };
 
-/* Running softmax of a lane's row: reference, this lane's part of the sum, O^T (d = 16 i + 4 g + r). */
+/* Running softmax of a lane's row: reference (and 0 or what takes a score off it), this lane's part of the
+ * sum, O^T (d = 16 i + 4 g + r). */
 template <int D>
 struct AttRow {
-    float ref, l;
-    f32x4 o[D / 16];
+    float ref = kLowest, neg = 0.0f, l = 0.0f;
+    f32x4 o[D / 16] = {};
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -164,38 +165,60 @@ struct AttP<0> {
     f32x4 v;
 };
 
-/* A row's step of the softmax: keys from `limit` on are hidden (left: limit less the lane's first key). */
-template <int TYPE, int D, bool MASK>
-__device__ __forceinline__ void soften(float c, int left, f32x4 (&s)[Att<TYPE, D>::TL], AttRow<D> &row, AttP<TYPE> &p)
+/* A step's scores of keys that the row does not see (left: its limit less the lane's first key). */
+template <int TL>
+__device__ __forceinline__ void hide(int left, f32x4 (&s)[TL])
+{
+#pragma unroll
+    for (int t = 0; t < TL; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[t][r] = 4 * t + r < left ? s[t][r] : kLowest;
+}
+
+/* Raise the references of NT row tiles for NS steps of scores where one is too far above its row's. */
+template <int D, int NT, int NS, int TL>
+__device__ __forceinline__ void raise(const float (&c)[NT], const f32x4 (&s)[NS][NT][TL], AttRow<D> (&row)[NT])
+{
+    float top[NT];
+    bool far = false;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        top[n] = s[0][n][0][0];
+#pragma unroll
+        for (int k = 0; k < NS; k++)
+#pragma unroll
+            for (int t = 0; t < TL; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) top[n] = fmaxf(top[n], s[k][n][t][r]);
+        top[n] *= c[n];
+        far = far || top[n] > row[n].ref + 14.0f;
+    }
+    if (__builtin_expect(__ballot(far) != 0, 0)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float ref = fmaxf(row[n].ref, row_max(top[n]) - 6.0f);
+            const float a = ref == row[n].ref ? 1.0f : exp2_fast(row[n].ref - ref);
+            row[n].ref = ref;
+            row[n].neg = ref == kLowest ? 0.0f : -ref;
+            row[n].l *= a;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) row[n].o[i] *= a;
+        }
+    }
+}
+
+/* A row's step of weights. */
+template <int TYPE, int D>
+__device__ __forceinline__ AttP<TYPE> soften(float c, f32x4 (&s)[Att<TYPE, D>::TL], AttRow<D> &row)
 {
     using A = Att<TYPE, D>;
-    if constexpr (MASK) {
-#pragma unroll
-        for (int t = 0; t < A::TL; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[t][r] = 4 * t + r < left ? s[t][r] : kLowest;
-    }
-    float top = s[0][0];
-#pragma unroll
-    for (int t = 0; t < A::TL; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) top = fmaxf(top, s[t][r]);
-    top *= c;
-    if (__builtin_expect(__ballot(top > row.ref + 14.0f) != 0, 0)) {
-        const float ref = fmaxf(row.ref, row_max(top) - 6.0f);
-        const float a = ref == row.ref ? 1.0f : exp2_fast(row.ref - ref);
-        row.ref = ref;
-        row.l *= a;
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) row.o[i] *= a;
-    }
-    const float nref = row.ref == kLowest ? 0.0f : -row.ref;
+    AttP<TYPE> p;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < A::TL; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], c, nref));
+            s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], c, row.neg));
             sum += s[t][r];
         }
     row.l += sum;
@@ -208,13 +231,15 @@ __device__ __forceinline__ void soften(float c, int left, f32x4 (&s)[Att<TYPE, D
             for (int r = 0; r < 4; r += 2) {
                 /* hi rounds towards zero: what it drops is in lo, to 11 more bits */
                 const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(s[t][r], s[t][r + 1]));
-                const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(s[t][r] - (float)hi.x, s[t][r + 1] - (float)hi.y));
+                const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.0f, s[t][r]),
+                                                                                __builtin_fmaf((float)hi.y, -1.0f, s[t][r + 1])));
                 p.hi[4 * t + r] = hi.x;
                 p.hi[4 * t + r + 1] = hi.y;
                 p.lo[4 * t + r] = lo.x;
                 p.lo[4 * t + r + 1] = lo.y;
             }
     }
+    return p;
 }
 
 /* Masks over the lane's piece of values: keys the item has (of n_key from the piece's first on), and of
@@ -365,10 +390,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
             const int t = any ? r / a.group : w.row / a.group;
             limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
             c[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
-            row[n].ref = kLowest;
-            row[n].l = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) row[n].o[i] = f32x4{ 0, 0, 0, 0 };
         }
         const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
         const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
@@ -404,20 +425,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
         for (int s = wave; s < n_step; s += kFewWaves) {
             const int key = w.key0 + s * A::KS;
             const bool more = s + kFewWaves < n_step, mask = key + A::KS > w.full;
-            f32x4 sc[NT][A::TL];
-            scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, sc);
+            f32x4 sc[1][NT][A::TL];
+            scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, sc[0]);
             if (more) load_k(s + kFewWaves);
-            AttP<TYPE> p[NT];
             if (mask) {
-#pragma unroll
-                for (int n = 0; n < NT; n++) soften<TYPE, D, true>(c[n], limit[n] - key - v_off, sc[n], row[n], p[n]);
+                hide(limit[0] - key - v_off, sc[0][0]);
                 const AttMask m = piece_mask<TYPE>(w.full - key - v_off, w.key1 - key - v_off);
 #pragma unroll
                 for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
-            } else {
-#pragma unroll
-                for (int n = 0; n < NT; n++) soften<TYPE, D, false>(c[n], 0, sc[n], row[n], p[n]);
             }
+            raise<D>(c, sc, row);
+            const AttP<TYPE> p[NT] = { soften<TYPE, D>(c[0], sc[0][0], row[0]) };
             weigh<TYPE, D, NT>([&](int i) { return vf[i]; }, p, row);
             if (more) {
                 load_v(s + kFewWaves);
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 /* Many rows (128): four waves of 32 rows each share tiles of keys and values, copied to LDS by the LDS
  * DMA, the next tile's copy in flight while one is worked on. Pieces are stored with their index in
  * the row xored by the row, so that the 16 rows a wave instruction reads lie in all banks. */
-constexpr int kManyNT = 1;
+constexpr int kManyNT = 2;
 constexpr int kManyThreads = 64 * 128 / (16 * kManyNT);
 
 template <int TYPE, int D>
@@ -509,17 +527,11 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
             head[n] = kvh * a.group + r % a.group;
             limit[n] = any ? min(toks[tok[n]].pos + 1, w.key1) : 0;
             c[n] = load_q<TYPE, D>(a.q + ((size_t)tok[n] * a.heads + head[n]) * D, any, g, a.scale_log2, q[n]);
-            row[n].ref = kLowest;
-            row[n].l = 0.0f;
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) row[n].o[k] = f32x4{ 0, 0, 0, 0 };
         }
         const int n_tile = (w.key1 - w.key0 + L::KT - 1) / L::KT, last = w.key1 - 1;
-        u32x4 pid;
-        auto pages = [&](int tile) {
-#pragma unroll
-            for (int i = 0; i < NG; i++) pid[i] = (uint32_t)__builtin_amdgcn_readfirstlane(tab[min(w.key0 + tile * L::KT + 16 * i, last) >> a.shift]);
-        };
+        /* lane i: the page of the next tile's keys 16 (i % NG) .., loaded a tile ahead of its use */
+        uint32_t pid = 0;
+        auto pages = [&](int tile) { pid = (uint32_t)tab[min(w.key0 + tile * L::KT + 16 * (lane % NG), last) >> a.shift]; };
         auto copy = [&](int tile) {
             const int key = w.key0 + tile * L::KT;
             uint8_t *kd = lds[tile & 1][0], *vd = lds[tile & 1][1];
@@ -528,9 +540,7 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
             for (int i = 0; i < NL; i++) {
                 const int r = i * RI + tid / RC;                     /* key row, and its 16 keys   */
                 const int grp = __builtin_amdgcn_readfirstlane(r / 16);
-                int pg = (int)pid[0];
-#pragma unroll
-                for (int k = 1; k < NG; k++) pg = grp == k ? (int)pid[k] : pg;
+                const int pg = __builtin_amdgcn_readlane(pid, grp);
                 const int m = TYPE == 1 ? (((r >> 3) & 3) << 2 | (r & 3)) : (r & 15);
                 const int piece = (tid % RC) ^ (m / RP);
                 const int slot = (key + r) & P1;
@@ -538,9 +548,9 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
                                kd + (i * kManyThreads + wave * 64) * 16);
             }
             const int piece = (tid & 7) ^ ((tid >> 4) & 7);
-            int pg = (int)pid[0];
+            int pg = __builtin_amdgcn_readlane(pid, 0);
 #pragma unroll
-            for (int k = 1; k < NG; k++) pg = piece * A::CE / 16 == k ? (int)pid[k] : pg;
+            for (int k = 1; k < NG; k++) pg = piece * A::CE / 16 == k ? __builtin_amdgcn_readlane(pid, k) : pg;
             const int slot = (key + piece * A::CE) & P1;
             const uint8_t *p = page_at(a.v, pg, a.page_bytes, head_off) + (uint32_t)(((tid >> 3) << a.shift) + slot) * A::ES;
             const uint32_t step = (uint32_t)(kManyThreads / 8 * A::ES) << a.shift;
@@ -561,29 +571,49 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
                 if (tile + 2 < n_tile) pages(tile + 2);
             }
         };
-        auto step = [&](auto masked, int tile, int st) {
+        /* steps of a tile, from st0 on: all their scores first, so that one branch serves them */
+        auto work_on = [&](auto masked, auto steps, int tile, int st0) {
             constexpr bool MASK = decltype(masked)::value;
-            const uint8_t *kr = lds[tile & 1][0] + (st * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
-            const uint8_t *vr = lds[tile & 1][1] + col * 128 + (((4 * st + g) ^ ((col >> 1) & 7)) * 16);
-            f32x4 sc[NT][A::TL];
-            scores<TYPE, D, NT>([&](int t, int i) { return *(const u32x4 *)(kr + 4 * t * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16)); }, q, sc);
-            AttP<TYPE> p[NT];
-            const int at = w.key0 + tile * L::KT + st * A::KS + g * A::CE;
+            constexpr int NS = decltype(steps)::value;
+            const uint8_t *kr = lds[tile & 1][0] + (st0 * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
+            const uint8_t *vr = lds[tile & 1][1] + col * 128;
+            const int at = w.key0 + tile * L::KT + st0 * A::KS + g * A::CE;
+            f32x4 sc[NS][NT][A::TL];
 #pragma unroll
-            for (int n = 0; n < NT; n++) soften<TYPE, D, MASK>(c[n], limit[n] - at, sc[n], row[n], p[n]);
-            if constexpr (MASK) {
-                const AttMask m = piece_mask<TYPE>(w.full - at, w.key1 - at);
-                weigh<TYPE, D, NT>([&](int i) { return clean<TYPE>(*(const u32x4 *)(vr + 2048 * i), m, bad); }, p, row);
-            } else {
-                weigh<TYPE, D, NT>([&](int i) { return *(const u32x4 *)(vr + 2048 * i); }, p, row);
+            for (int st = 0; st < NS; st++) {
+                u32x4 kf[A::NK];
+#pragma unroll
+                for (int i = 0; i < A::NCH; i++)
+#pragma unroll
+                    for (int t = 0; t < A::TL; t++)
+                        kf[t * A::NCH + i] = *(const u32x4 *)(kr + (st * A::KS + 4 * t) * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16));
+                scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, sc[st]);
+                if constexpr (MASK) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) hide(limit[n] - at - st * A::KS, sc[st][n]);
+                }
+            }
+            raise<D>(c, sc, row);
+#pragma unroll
+            for (int st = 0; st < NS; st++) {
+                u32x4 vf[A::NV];
+#pragma unroll
+                for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(vr + 2048 * i + (((4 * (st0 + st) + g) ^ ((col >> 1) & 7)) * 16));
+                AttP<TYPE> p[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) p[n] = soften<TYPE, D>(c[n], sc[st][n], row[n]);
+                if constexpr (MASK) {
+                    const AttMask m = piece_mask<TYPE>(w.full - at - st * A::KS, w.key1 - at - st * A::KS);
+#pragma unroll
+                    for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
+                }
+                weigh<TYPE, D, NT>([&](int i) { return vf[i]; }, p, row);
             }
         };
         const int n_clear = max(0, w.full - w.key0) / L::KT;        /* tiles that every row sees whole */
         for (int tile = 0; tile < n_clear; tile++) {
             turn(tile);
-            if (idle) continue;
-#pragma unroll
-            for (int st = 0; st < 2; st++) step(std::false_type{}, tile, st);
+            if (!idle) work_on(std::false_type{}, std::integral_constant<int, 2>{}, tile, 0);
         }
 #pragma unroll 1
         for (int tile = n_clear; tile < n_tile; tile++) {
@@ -591,7 +621,7 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
             if (idle) continue;
 #pragma unroll 1
             for (int st = 0; st < 2; st++)
-                if (w.key0 + tile * L::KT + st * A::KS < w.key1) step(std::true_type{}, tile, st);
+                if (w.key0 + tile * L::KT + st * A::KS < w.key1) work_on(std::true_type{}, std::integral_constant<int, 1>{}, tile, st);
         }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
