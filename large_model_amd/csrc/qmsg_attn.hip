@@ -13,14 +13,14 @@
  * neither a shuffle nor LDS on its way into the second product (CE elements in 16 bytes: 8 f16 in
  * two tiles a step of 32 keys, 4 f32 in one tile of 16).
  *
- * Activations are fp32. With an f16 cache q (scaled by a power of two so that its largest element
- * lies in [2^8, 2^9)) and p are split into two f16, x = hi + lo to 22 bits, and each product is two f16 MFMAs
+ * Activations are fp32. With an f16 cache q and p are split into two f16, x = hi + lo to 22 bits, and each product is two f16 MFMAs
  * into fp32: twice the f16 work, against the sixteenth of the rate that fp32 MFMAs would have. An fp32
  * cache takes the fp32 MFMAs as it is.
  *
- * Softmax in one pass: p = 2^(c s - ref) with ref a row's running reference, set 6 below the row's
+ * Softmax in one pass: p = 2^(s - ref) with s in powers of two (q is scaled) and ref a row's running reference, set 6 below the row's
  * largest score so far and raised only when a score passes it by 14, so that p stays below 2^14 (f16's
- * range) and the usual step needs no reduction across lanes. Sums, references and O are fp32. */
+ * range) and the usual step needs no reduction across lanes. The products' accumulators start at -ref, so
+ * that s - ref costs no instruction. Sums, references and O are fp32. */
 #include <cmath>
 #include <type_traits>
 
@@ -32,7 +32,6 @@ namespace qmsg {
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLowest = -INFINITY;
 
@@ -57,11 +56,11 @@ struct AttQ<0, D> {
     f32x4 v[Att<0, D>::NCH];
 };
 
-/* Running softmax of a lane's row: reference (and 0 or what takes a score off it), this lane's part of the
- * sum, O^T (d = 16 i + 4 g + r). */
+/* Running softmax of a lane's row: reference, this lane's part of the sum, O^T (d = 16 i + 4 g + r). What its
+ * scores are summed from (less the reference, in the units of the row's query) stands apart. */
 template <int D>
 struct AttRow {
-    float ref = kLowest, neg = 0.0f, l = 0.0f;
+    float ref = kLowest, l = 0.0f;
     f32x4 o[D / 16] = {};
 };
 
@@ -87,15 +86,17 @@ __device__ __forceinline__ float row_sum(float v)
     return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
-/* Load a row's query; returns what its scores are multiplied with to stand in powers of two. */
+/* Load a row's query times `scale`; returns the power of two that its scores come out multiplied with: 1 but
+ * for fp16 rows whose largest element is outside [2^-4, 2^14) (a row of zeros is inside). Those are
+ * scaled to [2^8, 2^9), so that neither half leaves f16's range. */
 template <int TYPE, int D>
-__device__ __forceinline__ float load_q(const float *row, bool any, int g, float scale_log2, AttQ<TYPE, D> &q)
+__device__ __forceinline__ float load_q(const float *row, bool any, int g, float scale, AttQ<TYPE, D> &q)
 {
     using A = Att<TYPE, D>;
     if constexpr (TYPE == 0) {
 #pragma unroll
-        for (int c = 0; c < A::NCH; c++) q.v[c] = any ? *(const f32x4 *)(row + 16 * c + 4 * g) : f32x4{ 0, 0, 0, 0 };
-        return scale_log2;
+        for (int c = 0; c < A::NCH; c++) q.v[c] = any ? *(const f32x4 *)(row + 16 * c + 4 * g) * scale : f32x4{ 0, 0, 0, 0 };
+        return 1.0f;
     } else {
         f32x4 x[A::NCH][2];
         float top = 0.0f;
@@ -103,15 +104,17 @@ __device__ __forceinline__ float load_q(const float *row, bool any, int g, float
         for (int c = 0; c < A::NCH; c++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                x[c][j] = any ? *(const f32x4 *)(row + 32 * c + 8 * g + 4 * j) : f32x4{ 0, 0, 0, 0 };
+                x[c][j] = any ? *(const f32x4 *)(row + 32 * c + 8 * g + 4 * j) * scale : f32x4{ 0, 0, 0, 0 };
 #pragma unroll
                 for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[c][j][e]));
             }
         top = row_max(top);
-        /* a row of zeros, of subnormals only or with an infinity keeps a scale inside fp32's range */
-        const int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-        const int sh = ex < -110 || ex > 127 ? 0 : 8 - ex;
-        const float up = __builtin_bit_cast(float, (uint32_t)(127 + sh) << 23), down = __builtin_bit_cast(float, (uint32_t)(127 - sh) << 23);
+        float up = 1.0f;
+        if (top != 0.0f && (top < 0.0625f || top >= 16384.0f)) {
+            /* subnormal rows and rows with an infinity keep a factor inside fp32's range */
+            const int ex = max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -110);
+            up = __builtin_bit_cast(float, (uint32_t)(127 + 8 - min(ex, 127)) << 23);
+        }
 #pragma unroll
         for (int c = 0; c < A::NCH; c++)
 #pragma unroll
@@ -121,19 +124,20 @@ __device__ __forceinline__ float load_q(const float *row, bool any, int g, float
                 q.hi[c][e] = hi;
                 q.lo[c][e] = (_Float16)(v - (float)hi);
             }
-        return scale_log2 * down;
+        return up;
     }
 }
 
-/* One step's scores of NT row tiles: s[n][tl][r] of key g * CE + 4 tl + r. key(tl, c): the lane's piece. */
+/* One step's scores of NT row tiles off their references: s[n][tl][r] of key g * CE + 4 tl + r. key(tl, c): the
+ * lane's piece. */
 template <int TYPE, int D, int NT, class K>
-__device__ __forceinline__ void scores(K key, const AttQ<TYPE, D> (&q)[NT], f32x4 (&s)[NT][Att<TYPE, D>::TL])
+__device__ __forceinline__ void scores(K key, const AttQ<TYPE, D> (&q)[NT], const float (&from)[NT], f32x4 (&s)[NT][Att<TYPE, D>::TL])
 {
     using A = Att<TYPE, D>;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int t = 0; t < A::TL; t++) s[n][t] = f32x4{ 0, 0, 0, 0 };
+        for (int t = 0; t < A::TL; t++) s[n][t] = f32x4{ from[n], from[n], from[n], from[n] };
 #pragma unroll
     for (int c = 0; c < A::NCH; c++)
 #pragma unroll
@@ -165,6 +169,20 @@ struct AttP<0> {
     f32x4 v;
 };
 
+/* Scores of rows whose query was scaled up, taken back down. */
+template <int NT, int NS, int TL>
+__device__ __forceinline__ void unscale(const float (&up)[NT], f32x4 (&s)[NS][NT][TL])
+{
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float down = 1.0f / up[n];                     /* powers of two */
+#pragma unroll
+        for (int k = 0; k < NS; k++)
+#pragma unroll
+            for (int t = 0; t < TL; t++) s[k][n][t] *= down;
+    }
+}
+
 /* A step's scores of keys that the row does not see (left: its limit less the lane's first key). */
 template <int TL>
 __device__ __forceinline__ void hide(int left, f32x4 (&s)[TL])
@@ -175,9 +193,10 @@ __device__ __forceinline__ void hide(int left, f32x4 (&s)[TL])
         for (int r = 0; r < 4; r++) s[t][r] = 4 * t + r < left ? s[t][r] : kLowest;
 }
 
-/* Raise the references of NT row tiles for NS steps of scores where one is too far above its row's. */
+/* Raise the references of NT row tiles for NS steps of scores (off their references) where one is too far
+ * above its row's. */
 template <int D, int NT, int NS, int TL>
-__device__ __forceinline__ void raise(const float (&c)[NT], const f32x4 (&s)[NS][NT][TL], AttRow<D> (&row)[NT])
+__device__ __forceinline__ void raise(const float (&up)[NT], f32x4 (&s)[NS][NT][TL], float (&from)[NT], AttRow<D> (&row)[NT])
 {
     float top[NT];
     bool far = false;
@@ -190,26 +209,42 @@ __device__ __forceinline__ void raise(const float (&c)[NT], const f32x4 (&s)[NS]
             for (int t = 0; t < TL; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) top[n] = fmaxf(top[n], s[k][n][t][r]);
-        top[n] *= c[n];
-        far = far || top[n] > row[n].ref + 14.0f;
+        /* a row without a reference has its scores as they are */
+        far = far || top[n] > (row[n].ref == kLowest ? kLowest : 14.0f);
     }
     if (__builtin_expect(__ballot(far) != 0, 0)) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const float ref = fmaxf(row[n].ref, row_max(top[n]) - 6.0f);
+            const float base = row[n].ref == kLowest ? 0.0f : row[n].ref;
+            const float ref = fmaxf(row[n].ref, base + row_max(top[n]) - 6.0f);
             const float a = ref == row[n].ref ? 1.0f : exp2_fast(row[n].ref - ref);
+            const float off = ref == kLowest ? 0.0f : base - ref;
             row[n].ref = ref;
-            row[n].neg = ref == kLowest ? 0.0f : -ref;
+            from[n] = ref == kLowest ? 0.0f : -ref * up[n];
             row[n].l *= a;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) row[n].o[i] *= a;
+#pragma unroll
+            for (int k = 0; k < NS; k++)
+#pragma unroll
+                for (int t = 0; t < TL; t++) s[k][n][t] += off;
         }
     }
 }
 
+/* x - (float)half I of h, in one instruction. */
+template <int I>
+__device__ __forceinline__ float less_half(float x, uint32_t h)
+{
+    float r;
+    if constexpr (I == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+
 /* A row's step of weights. */
 template <int TYPE, int D>
-__device__ __forceinline__ AttP<TYPE> soften(float c, f32x4 (&s)[Att<TYPE, D>::TL], AttRow<D> &row)
+__device__ __forceinline__ AttP<TYPE> soften(AttRow<D> &row, f32x4 (&s)[Att<TYPE, D>::TL])
 {
     using A = Att<TYPE, D>;
     AttP<TYPE> p;
@@ -218,26 +253,23 @@ __device__ __forceinline__ AttP<TYPE> soften(float c, f32x4 (&s)[Att<TYPE, D>::T
     for (int t = 0; t < A::TL; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], c, row.neg));
+            s[t][r] = exp2_fast(s[t][r]);
             sum += s[t][r];
         }
     row.l += sum;
     if constexpr (TYPE == 0) {
         p.v = s[0];
     } else {
+        /* hi rounds towards zero: what it drops is in lo, to 11 more bits */
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int t = 0; t < A::TL; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r += 2) {
-                /* hi rounds towards zero: what it drops is in lo, to 11 more bits */
-                const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(s[t][r], s[t][r + 1]));
-                const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.0f, s[t][r]),
-                                                                                __builtin_fmaf((float)hi.y, -1.0f, s[t][r + 1])));
-                p.hi[4 * t + r] = hi.x;
-                p.hi[4 * t + r + 1] = hi.y;
-                p.lo[4 * t + r] = lo.x;
-                p.lo[4 * t + r + 1] = lo.y;
-            }
+        for (int i = 0; i < 4; i++) {
+            const float x = s[i / 2][2 * (i % 2)], y = s[i / 2][2 * (i % 2) + 1];
+            hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+            lo[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x, hi[i]), less_half<1>(y, hi[i])));
+        }
+        p.hi = __builtin_bit_cast(h8, u32x4{ hi[0], hi[1], hi[2], hi[3] });
+        p.lo = __builtin_bit_cast(h8, u32x4{ lo[0], lo[1], lo[2], lo[3] });
     }
     return p;
 }
@@ -381,7 +413,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
         AttQ<TYPE, D> q[NT];
         AttRow<D> row[NT];
-        float c[NT];
+        float up[NT], from[NT] = {};
         int limit[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -389,8 +421,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
             const bool any = 16 * n + col < w.rows;
             const int t = any ? r / a.group : w.row / a.group;
             limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
-            c[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
+            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
         }
+        const bool unit = __ballot(up[0] != 1.0f) == 0;
         const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
         const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
         u32x4 kf[A::NK], vf[A::NV];
@@ -426,7 +459,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
             const int key = w.key0 + s * A::KS;
             const bool more = s + kFewWaves < n_step, mask = key + A::KS > w.full;
             f32x4 sc[1][NT][A::TL];
-            scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, sc[0]);
+            scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, from, sc[0]);
+            if (!unit) unscale(up, sc);
             if (more) load_k(s + kFewWaves);
             if (mask) {
                 hide(limit[0] - key - v_off, sc[0][0]);
@@ -434,8 +468,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 #pragma unroll
                 for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
             }
-            raise<D>(c, sc, row);
-            const AttP<TYPE> p[NT] = { soften<TYPE, D>(c[0], sc[0][0], row[0]) };
+            raise(up, sc, from, row);
+            const AttP<TYPE> p[NT] = { soften<TYPE, D>(row[0], sc[0][0]) };
             weigh<TYPE, D, NT>([&](int i) { return vf[i]; }, p, row);
             if (more) {
                 load_v(s + kFewWaves);
@@ -517,21 +551,30 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
         AttQ<TYPE, D> q[NT];
         AttRow<D> row[NT];
-        float c[NT];
-        int limit[NT], tok[NT], head[NT];
+        float up[NT], from[NT] = {};
+        int limit[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int i = 16 * NT * wave + 16 * n + col, r = w.row + i;
             const bool any = i < w.rows;
-            tok[n] = any ? r / a.group : w.row / a.group;
-            head[n] = kvh * a.group + r % a.group;
-            limit[n] = any ? min(toks[tok[n]].pos + 1, w.key1) : 0;
-            c[n] = load_q<TYPE, D>(a.q + ((size_t)tok[n] * a.heads + head[n]) * D, any, g, a.scale_log2, q[n]);
+            const int t = any ? r / a.group : w.row / a.group;
+            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
+            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
         }
+        bool scaled = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) scaled = scaled || up[n] != 1.0f;
+        const bool unit = __ballot(scaled) == 0;
         const int n_tile = (w.key1 - w.key0 + L::KT - 1) / L::KT, last = w.key1 - 1;
-        /* lane i: the page of the next tile's keys 16 (i % NG) .., loaded a tile ahead of its use */
-        uint32_t pid = 0;
-        auto pages = [&](int tile) { pid = (uint32_t)tab[min(w.key0 + tile * L::KT + 16 * (lane % NG), last) >> a.shift]; };
+        /* the next tile's pages, loaded a tile ahead of their use: in lane i the page of keys 16 (i % NG) ..,
+         * and the one of the values that the thread copies */
+        const int v_piece = (tid & 7) ^ ((tid >> 4) & 7);
+        int k_page = 0, v_page = 0;
+        auto pages = [&](int tile) {
+            const int key = w.key0 + tile * L::KT;
+            k_page = tab[min(key + 16 * (lane % NG), last) >> a.shift];
+            v_page = tab[min(key + v_piece * A::CE, last) >> a.shift];
+        };
         auto copy = [&](int tile) {
             const int key = w.key0 + tile * L::KT;
             uint8_t *kd = lds[tile & 1][0], *vd = lds[tile & 1][1];
@@ -539,20 +582,15 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int r = i * RI + tid / RC;                     /* key row, and its 16 keys   */
-                const int grp = __builtin_amdgcn_readfirstlane(r / 16);
-                const int pg = __builtin_amdgcn_readlane(pid, grp);
+                const int pg = __builtin_amdgcn_readlane(k_page, (i * RI + wave * (64 / RC)) / 16);
                 const int m = TYPE == 1 ? (((r >> 3) & 3) << 2 | (r & 3)) : (r & 15);
                 const int piece = (tid % RC) ^ (m / RP);
                 const int slot = (key + r) & P1;
                 dma_to_lds<16>(page_at(a.k, pg, a.page_bytes, head_off) + (uint32_t)(slot * D + piece * A::CE) * A::ES,
                                kd + (i * kManyThreads + wave * 64) * 16);
             }
-            const int piece = (tid & 7) ^ ((tid >> 4) & 7);
-            int pg = __builtin_amdgcn_readlane(pid, 0);
-#pragma unroll
-            for (int k = 1; k < NG; k++) pg = piece * A::CE / 16 == k ? __builtin_amdgcn_readlane(pid, k) : pg;
-            const int slot = (key + piece * A::CE) & P1;
-            const uint8_t *p = page_at(a.v, pg, a.page_bytes, head_off) + (uint32_t)(((tid >> 3) << a.shift) + slot) * A::ES;
+            const int slot = (key + v_piece * A::CE) & P1;
+            const uint8_t *p = page_at(a.v, v_page, a.page_bytes, head_off) + (uint32_t)(((tid >> 3) << a.shift) + slot) * A::ES;
             const uint32_t step = (uint32_t)(kManyThreads / 8 * A::ES) << a.shift;
 #pragma unroll
             for (int i = 0; i < NL; i++) dma_to_lds<16>(p + i * step, vd + (i * kManyThreads + wave * 64) * 16);
@@ -587,13 +625,16 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
 #pragma unroll
                     for (int t = 0; t < A::TL; t++)
                         kf[t * A::NCH + i] = *(const u32x4 *)(kr + (st * A::KS + 4 * t) * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16));
-                scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, sc[st]);
-                if constexpr (MASK) {
+                scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, from, sc[st]);
+            }
+            if (!unit) unscale(up, sc);
+            if constexpr (MASK) {
+#pragma unroll
+                for (int st = 0; st < NS; st++)
 #pragma unroll
                     for (int n = 0; n < NT; n++) hide(limit[n] - at - st * A::KS, sc[st][n]);
-                }
             }
-            raise<D>(c, sc, row);
+            raise(up, sc, from, row);
 #pragma unroll
             for (int st = 0; st < NS; st++) {
                 u32x4 vf[A::NV];
@@ -601,7 +642,7 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
                 for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(vr + 2048 * i + (((4 * (st0 + st) + g) ^ ((col >> 1) & 7)) * 16));
                 AttP<TYPE> p[NT];
 #pragma unroll
-                for (int n = 0; n < NT; n++) p[n] = soften<TYPE, D>(c[n], sc[st][n], row[n]);
+                for (int n = 0; n < NT; n++) p[n] = soften<TYPE, D>(row[n], sc[st][n]);
                 if constexpr (MASK) {
                     const AttMask m = piece_mask<TYPE>(w.full - at - st * A::KS, w.key1 - at - st * A::KS);
 #pragma unroll
@@ -626,13 +667,14 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const float l = row_sum(row[n].l);
-            if (16 * NT * wave + 16 * n + col >= w.rows) continue;
-            const AttnTok tk = toks[tok[n]];
+            const int i = 16 * NT * wave + 16 * n + col, r = w.row + i, t = r / a.group, head = kvh * a.group + r % a.group;
+            if (i >= w.rows) continue;
+            const AttnTok tk = toks[t];
 #pragma unroll
-            for (int i = 0; i < D / 16; i++)
-                put_row(a, tk, w.part, tok[n], head[n], 16 * i + 4 * g, D, row[n].ref, l, row[n].o[i], i == 0 && g == 0);
+            for (int k = 0; k < D / 16; k++)
+                put_row(a, tk, w.part, t, head, 16 * k + 4 * g, D, row[n].ref, l, row[n].o[k], k == 0 && g == 0);
             if (__builtin_expect(__ballot(bad) != 0, 0)) {
-                float *o = row_out(a, tk, w.part, tok[n], head[n], D);
+                float *o = row_out(a, tk, w.part, t, head, D);
 #pragma unroll 1
                 for (int d = 4 * g; d < D; d += 16) {
                     const f32x4 e = wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, limit[n], d);
