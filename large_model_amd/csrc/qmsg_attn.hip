@@ -128,45 +128,43 @@ __device__ __forceinline__ float load_q(const float *row, bool any, int g, float
     }
 }
 
-/* One step's scores of NT row tiles off their references: s[n][tl][r] of key g * CE + 4 tl + r. key(tl, c): the
- * lane's piece. */
-template <int TYPE, int D, int NT, class K>
-__device__ __forceinline__ void scores(K key, const AttQ<TYPE, D> (&q)[NT], const float (&from)[NT], f32x4 (&s)[NT][Att<TYPE, D>::TL])
+/* A piece of keys (piece c of tile t) times NT rows, into their scores. */
+template <int TYPE, int D, int NT>
+__device__ __forceinline__ void score(u32x4 k, int c, int t, const AttQ<TYPE, D> (&q)[NT], f32x4 (&s)[NT][Att<TYPE, D>::TL])
 {
-    using A = Att<TYPE, D>;
+    if constexpr (TYPE == 0) {
+        const f32x4 x = __builtin_bit_cast(f32x4, k);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[n].v[c][e], s[n][t], 0, 0, 0);
+    } else {
+        const h8 x = __builtin_bit_cast(h8, k);
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].lo[c], s[n][t], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].hi[c], s[n][t], 0, 0, 0);
+    }
+}
+
+/* A step's scores s[n][t][r] of key g * CE + 4 t + r start at `from`: they come out off their references. */
+template <int NT, int TL>
+__device__ __forceinline__ void score_from(const float (&from)[NT], f32x4 (&s)[NT][TL])
+{
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int t = 0; t < A::TL; t++) s[n][t] = f32x4{ from[n], from[n], from[n], from[n] };
-#pragma unroll
-    for (int c = 0; c < A::NCH; c++)
-#pragma unroll
-        for (int t = 0; t < A::TL; t++) {
-            const u32x4 k = key(t, c);
-            if constexpr (TYPE == 0) {
-                const f32x4 x = __builtin_bit_cast(f32x4, k);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[n].v[c][e], s[n][t], 0, 0, 0);
-            } else {
-                const h8 x = __builtin_bit_cast(h8, k);
-#pragma unroll
-                for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].lo[c], s[n][t], 0, 0, 0);
-#pragma unroll
-                for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].hi[c], s[n][t], 0, 0, 0);
-            }
-        }
+        for (int t = 0; t < TL; t++) s[n][t] = f32x4{ from[n], from[n], from[n], from[n] };
 }
 
-/* P as B operand. */
+/* P as B operand: two f16 of each weight, or the weights. */
 template <int TYPE>
 struct AttP {
-    h8 hi, lo;
+    uint32_t hi[4], lo[4];
 };
 template <>
 struct AttP<0> {
-    f32x4 v;
+    float v[4];
 };
 
 /* Scores of rows whose query was scaled up, taken back down. */
@@ -242,36 +240,26 @@ __device__ __forceinline__ float less_half(float x, uint32_t h)
     return r;
 }
 
-/* A row's step of weights. */
+/* The weights of key tile t of a row's step, from its scores. */
 template <int TYPE, int D>
-__device__ __forceinline__ AttP<TYPE> soften(AttRow<D> &row, f32x4 (&s)[Att<TYPE, D>::TL])
+__device__ __forceinline__ void soften(int t, f32x4 s, AttRow<D> &row, AttP<TYPE> &p)
 {
-    using A = Att<TYPE, D>;
-    AttP<TYPE> p;
-    float sum = 0.0f;
+    float x[4];
 #pragma unroll
-    for (int t = 0; t < A::TL; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            s[t][r] = exp2_fast(s[t][r]);
-            sum += s[t][r];
-        }
-    row.l += sum;
+    for (int r = 0; r < 4; r++) x[r] = exp2_fast(s[r]);
+    row.l += (x[0] + x[1]) + (x[2] + x[3]);
     if constexpr (TYPE == 0) {
-        p.v = s[0];
+#pragma unroll
+        for (int r = 0; r < 4; r++) p.v[r] = x[r];
     } else {
         /* hi rounds towards zero: what it drops is in lo, to 11 more bits */
-        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float x = s[i / 2][2 * (i % 2)], y = s[i / 2][2 * (i % 2) + 1];
-            hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
-            lo[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x, hi[i]), less_half<1>(y, hi[i])));
+        for (int i = 0; i < 2; i++) {
+            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
+            p.hi[2 * t + i] = h;
+            p.lo[2 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x[2 * i], h), less_half<1>(x[2 * i + 1], h)));
         }
-        p.hi = __builtin_bit_cast(h8, u32x4{ hi[0], hi[1], hi[2], hi[3] });
-        p.lo = __builtin_bit_cast(h8, u32x4{ lo[0], lo[1], lo[2], lo[3] });
     }
-    return p;
 }
 
 /* Masks over the lane's piece of values: keys the item has (of n_key from the piece's first on), and of
@@ -318,25 +306,24 @@ __device__ __forceinline__ u32x4 clean(u32x4 v, const AttMask &m, uint32_t &bad)
     return v;
 }
 
-/* O^T += V^T P^T for NT row tiles. V(i): the lane's piece of values d = 16 i + col. */
-template <int TYPE, int D, int NT, class V>
-__device__ __forceinline__ void weigh(V val, const AttP<TYPE> (&p)[NT], AttRow<D> (&row)[NT])
+/* O^T += V^T P^T of NT rows for the piece v of values d = 16 i + col. */
+template <int TYPE, int D, int NT>
+__device__ __forceinline__ void weigh(u32x4 v, int i, const AttP<TYPE> (&p)[NT], AttRow<D> (&row)[NT])
 {
+    if constexpr (TYPE == 0) {
+        const f32x4 x = __builtin_bit_cast(f32x4, v);
 #pragma unroll
-    for (int i = 0; i < D / 16; i++) {
-        const u32x4 v = val(i);
+        for (int e = 0; e < 4; e++)
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            if constexpr (TYPE == 0) {
-                const f32x4 x = __builtin_bit_cast(f32x4, v);
+            for (int n = 0; n < NT; n++) row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[n].v[e], row[n].o[i], 0, 0, 0);
+    } else {
+        const h8 x = __builtin_bit_cast(h8, v);
 #pragma unroll
-                for (int e = 0; e < 4; e++) row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[n].v[e], row[n].o[i], 0, 0, 0);
-            } else {
-                const h8 x = __builtin_bit_cast(h8, v);
-                row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[n].hi, row[n].o[i], 0, 0, 0);
-                row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[n].lo, row[n].o[i], 0, 0, 0);
-            }
-        }
+        for (int n = 0; n < NT; n++)
+            row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, u32x4{ p[n].hi[0], p[n].hi[1], p[n].hi[2], p[n].hi[3] }), row[n].o[i], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+            row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, u32x4{ p[n].lo[0], p[n].lo[1], p[n].lo[2], p[n].lo[3] }), row[n].o[i], 0, 0, 0);
     }
 }
 
@@ -411,19 +398,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
         const int kvh = item % a.kv_heads;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
-        AttQ<TYPE, D> q[NT];
-        AttRow<D> row[NT];
-        float up[NT], from[NT] = {};
-        int limit[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int r = w.row + 16 * n + col;
-            const bool any = 16 * n + col < w.rows;
-            const int t = any ? r / a.group : w.row / a.group;
-            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
-            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
-        }
-        const bool unit = __ballot(up[0] != 1.0f) == 0;
         const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
         const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
         u32x4 kf[A::NK], vf[A::NV];
@@ -455,11 +429,28 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
             load_v(wave);
             if (wave + kFewWaves < n_step) pages(wave + kFewWaves);
         }
+        AttQ<TYPE, D> q[NT];
+        AttRow<D> row[NT];
+        float up[NT], from[NT] = {};
+        int limit[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int r = w.row + 16 * n + col;
+            const bool any = 16 * n + col < w.rows;
+            const int t = any ? r / a.group : w.row / a.group;
+            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
+            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
+        }
+        const bool unit = __ballot(up[0] != 1.0f) == 0;
         for (int s = wave; s < n_step; s += kFewWaves) {
             const int key = w.key0 + s * A::KS;
             const bool more = s + kFewWaves < n_step, mask = key + A::KS > w.full;
             f32x4 sc[1][NT][A::TL];
-            scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, from, sc[0]);
+            score_from(from, sc[0]);
+#pragma unroll
+            for (int i = 0; i < A::NCH; i++)
+#pragma unroll
+                for (int t = 0; t < A::TL; t++) score<TYPE, D, NT>(kf[t * A::NCH + i], i, t, q, sc[0]);
             if (!unit) unscale(up, sc);
             if (more) load_k(s + kFewWaves);
             if (mask) {
@@ -469,8 +460,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
                 for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
             }
             raise(up, sc, from, row);
-            const AttP<TYPE> p[NT] = { soften<TYPE, D>(row[0], sc[0][0]) };
-            weigh<TYPE, D, NT>([&](int i) { return vf[i]; }, p, row);
+            AttP<TYPE> p[NT];
+#pragma unroll
+            for (int t = 0; t < A::TL; t++) soften<TYPE, D>(t, sc[0][0][t], row[0], p[0]);
+#pragma unroll
+            for (int i = 0; i < A::NV; i++) weigh<TYPE, D, NT>(vf[i], i, p, row);
             if (more) {
                 load_v(s + kFewWaves);
                 if (s + 2 * kFewWaves < n_step) pages(s + 2 * kFewWaves);
@@ -549,22 +543,6 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
         const int kvh = item % a.kv_heads;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
-        AttQ<TYPE, D> q[NT];
-        AttRow<D> row[NT];
-        float up[NT], from[NT] = {};
-        int limit[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int i = 16 * NT * wave + 16 * n + col, r = w.row + i;
-            const bool any = i < w.rows;
-            const int t = any ? r / a.group : w.row / a.group;
-            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
-            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
-        }
-        bool scaled = false;
-#pragma unroll
-        for (int n = 0; n < NT; n++) scaled = scaled || up[n] != 1.0f;
-        const bool unit = __ballot(scaled) == 0;
         const int n_tile = (w.key1 - w.key0 + L::KT - 1) / L::KT, last = w.key1 - 1;
         /* the next tile's pages, loaded a tile ahead of their use: in lane i the page of keys 16 (i % NG) ..,
          * and the one of the values that the thread copies */
@@ -595,13 +573,29 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
 #pragma unroll
             for (int i = 0; i < NL; i++) dma_to_lds<16>(p + i * step, vd + (i * kManyThreads + wave * 64) * 16);
         };
-        uint32_t bad = 0;
-        const bool idle = 16 * NT * wave >= w.rows;
-        if (n_tile > 0) {
+        if (n_tile > 0) {                                           /* before the queries, which take as long to arrive */
             pages(0);
             copy(0);
             if (n_tile > 1) pages(1);
         }
+        uint32_t bad = 0;
+        const bool idle = 16 * NT * wave >= w.rows;
+        AttQ<TYPE, D> q[NT];
+        AttRow<D> row[NT];
+        float up[NT], from[NT] = {};
+        int limit[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int i = 16 * NT * wave + 16 * n + col, r = w.row + i;
+            const bool any = i < w.rows;
+            const int t = any ? r / a.group : w.row / a.group;
+            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
+            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
+        }
+        bool scaled = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) scaled = scaled || up[n] != 1.0f;
+        const bool unit = __ballot(scaled) == 0;
         auto turn = [&](int tile) {                                 /* tile's copy is there, the next one starts */
             mx_wait_barrier();
             if (tile + 1 < n_tile) {
@@ -609,24 +603,42 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
                 if (tile + 2 < n_tile) pages(tile + 2);
             }
         };
-        /* steps of a tile, from st0 on: all their scores first, so that one branch serves them */
+        /* Steps of a tile, from st0 on: all their scores first, so that one branch serves them. LDS reads run two
+         * pieces of keys and four of values ahead of their products, and a step's softmax between the
+         * products of the one before; the barriers keep the compiler from undoing that. */
         auto work_on = [&](auto masked, auto steps, int tile, int st0) {
             constexpr bool MASK = decltype(masked)::value;
-            constexpr int NS = decltype(steps)::value;
+            constexpr int NS = decltype(steps)::value, GK = NS * A::NCH, GV = NS * A::NV, KB = 3, VB = 4;
             const uint8_t *kr = lds[tile & 1][0] + (st0 * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
             const uint8_t *vr = lds[tile & 1][1] + col * 128;
             const int at = w.key0 + tile * L::KT + st0 * A::KS + g * A::CE;
             f32x4 sc[NS][NT][A::TL];
+            u32x4 kb[KB][A::TL], vb[VB];
+            auto read_k = [&](int j) {
 #pragma unroll
-            for (int st = 0; st < NS; st++) {
-                u32x4 kf[A::NK];
+                for (int t = 0; t < A::TL; t++)
+                    kb[j % KB][t] = *(const u32x4 *)(kr + (j / A::NCH * A::KS + 4 * t) * D * A::ES + (((4 * (j % A::NCH) + g) ^ (col / RP)) * 16));
+            };
+            auto read_v = [&](int j) { vb[j % VB] = *(const u32x4 *)(vr + 2048 * (j % A::NV) + (((4 * (st0 + j / A::NV) + g) ^ ((col >> 1) & 7)) * 16)); };
+            AttP<TYPE> p[2][NT];
+            constexpr int PARTS = NT * A::TL;                       /* of a step's softmax */
+            auto soft = [&](int st, int k) { soften<TYPE, D>(k % A::TL, sc[st][k / A::TL][k % A::TL], row[k / A::TL], p[st % 2][k / A::TL]); };
+            __builtin_amdgcn_s_setprio(1);                          /* over the SIMD's other wave where that has its softmax */
 #pragma unroll
-                for (int i = 0; i < A::NCH; i++)
+            for (int st = 0; st < NS; st++) score_from(from, sc[st]);
 #pragma unroll
-                    for (int t = 0; t < A::TL; t++)
-                        kf[t * A::NCH + i] = *(const u32x4 *)(kr + (st * A::KS + 4 * t) * D * A::ES + (((4 * i + g) ^ (col / RP)) * 16));
-                scores<TYPE, D, NT>([&](int t, int i) { return kf[t * A::NCH + i]; }, q, from, sc[st]);
+            for (int j = 0; j < KB - 1; j++) read_k(j);
+#pragma unroll
+            for (int j = 0; j < GK; j++) {
+                if (j + KB - 1 < GK) read_k(j + KB - 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < A::TL; t++) score<TYPE, D, NT>(kb[j % KB][t], j % A::NCH, t, q, sc[j / A::NCH]);
             }
+#pragma unroll
+            for (int j = 0; j < VB; j++) read_v(j);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             if (!unit) unscale(up, sc);
             if constexpr (MASK) {
 #pragma unroll
@@ -636,20 +648,19 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
             }
             raise(up, sc, from, row);
 #pragma unroll
-            for (int st = 0; st < NS; st++) {
-                u32x4 vf[A::NV];
+            for (int k = 0; k < PARTS; k++) soft(0, k);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(vr + 2048 * i + (((4 * (st0 + st) + g) ^ ((col >> 1) & 7)) * 16));
-                AttP<TYPE> p[NT];
-#pragma unroll
-                for (int n = 0; n < NT; n++) p[n] = soften<TYPE, D>(row[n], sc[st][n]);
-                if constexpr (MASK) {
-                    const AttMask m = piece_mask<TYPE>(w.full - at - st * A::KS, w.key1 - at - st * A::KS);
-#pragma unroll
-                    for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
-                }
-                weigh<TYPE, D, NT>([&](int i) { return vf[i]; }, p, row);
+            for (int j = 0; j < GV; j++) {
+                const int st = j / A::NV, i = j % A::NV;
+                u32x4 v = vb[j % VB];
+                if constexpr (MASK) v = clean<TYPE>(v, piece_mask<TYPE>(w.full - at - st * A::KS, w.key1 - at - st * A::KS), bad);
+                weigh<TYPE, D, NT>(v, i, p[st % 2], row);
+                if (j + VB < GV) read_v(j + VB);
+                if (st + 1 < NS && i % (A::NV / PARTS) == 0) soft(st + 1, i / (A::NV / PARTS));
+                __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
         };
         const int n_clear = max(0, w.full - w.key0) / L::KT;        /* tiles that every row sees whole */
         for (int tile = 0; tile < n_clear; tile++) {
