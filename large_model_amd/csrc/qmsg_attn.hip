@@ -86,44 +86,72 @@ __device__ __forceinline__ float row_sum(float v)
     return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
-/* Load a row's query times `scale`; returns the power of two that its scores come out multiplied with: 1 but
- * for fp16 rows whose largest element is outside [2^-4, 2^14) (a row of zeros is inside). Those are
+/* A row's query as it lies in memory, 16 bytes a load. */
+template <int TYPE, int D>
+struct AttRaw {
+    f32x4 x[D / 16];
+};
+template <int TYPE, int D>
+__device__ __forceinline__ void load_q(const float *row, int g, AttRaw<TYPE, D> &raw)
+{
+    constexpr int CE = Att<TYPE, D>::CE;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) raw.x[i] = *(const f32x4 *)(row + i / (CE / 4) * 4 * CE + CE * g + i % (CE / 4) * 4);
+}
+
+/* x - (float)half I of h, in one instruction. */
+template <int I>
+__device__ __forceinline__ float less_half(float x, uint32_t h)
+{
+    float r;
+    if constexpr (I == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+
+/* x and y as two f16 each. hi rounds towards zero: what it drops is in lo, to 11 more bits. */
+__device__ __forceinline__ void split(float x, float y, uint32_t &hi, uint32_t &lo)
+{
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x, hi), less_half<1>(y, hi)));
+}
+
+/* A query times `scale` as B operand; returns the power of two that its scores come out multiplied with: 1
+ * but for fp16 rows whose largest element is outside [2^-4, 2^14) (a row of zeros is inside). Those are
  * scaled to [2^8, 2^9), so that neither half leaves f16's range. */
 template <int TYPE, int D>
-__device__ __forceinline__ float load_q(const float *row, bool any, int g, float scale, AttQ<TYPE, D> &q)
+__device__ __forceinline__ float make_q(AttRaw<TYPE, D> &raw, float scale, AttQ<TYPE, D> &q)
 {
     using A = Att<TYPE, D>;
     if constexpr (TYPE == 0) {
 #pragma unroll
-        for (int c = 0; c < A::NCH; c++) q.v[c] = any ? *(const f32x4 *)(row + 16 * c + 4 * g) * scale : f32x4{ 0, 0, 0, 0 };
+        for (int c = 0; c < A::NCH; c++) q.v[c] = raw.x[c] * scale;
         return 1.0f;
     } else {
-        f32x4 x[A::NCH][2];
-        float top = 0.0f;
+        float top = 0.0f, up = 1.0f;
 #pragma unroll
-        for (int c = 0; c < A::NCH; c++)
+        for (int i = 0; i < D / 16; i++) {
+            raw.x[i] *= scale;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                x[c][j] = any ? *(const f32x4 *)(row + 32 * c + 8 * g + 4 * j) * scale : f32x4{ 0, 0, 0, 0 };
-#pragma unroll
-                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[c][j][e]));
-            }
+            for (int e = 0; e < 4; e += 2) top = fmaxf(top, fmaxf(fabsf(raw.x[i][e]), fabsf(raw.x[i][e + 1])));
+        }
         top = row_max(top);
-        float up = 1.0f;
-        if (top != 0.0f && (top < 0.0625f || top >= 16384.0f)) {
+        const bool far = top != 0.0f && (top < 0.0625f || top >= 16384.0f);
+        if (__ballot(far)) {
             /* subnormal rows and rows with an infinity keep a factor inside fp32's range */
-            const int ex = max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -110);
-            up = __builtin_bit_cast(float, (uint32_t)(127 + 8 - min(ex, 127)) << 23);
+            const int ex = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -110), 127);
+            if (far) up = __builtin_bit_cast(float, (uint32_t)(127 + 8 - ex) << 23);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) raw.x[i] *= up;
         }
 #pragma unroll
-        for (int c = 0; c < A::NCH; c++)
+        for (int c = 0; c < A::NCH; c++) {
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = x[c][e / 4][e % 4] * up;
-                const _Float16 hi = (_Float16)v;
-                q.hi[c][e] = hi;
-                q.lo[c][e] = (_Float16)(v - (float)hi);
-            }
+            for (int k = 0; k < 4; k++) split(raw.x[2 * c + k / 2][2 * (k % 2)], raw.x[2 * c + k / 2][2 * (k % 2) + 1], hi[k], lo[k]);
+            q.hi[c] = __builtin_bit_cast(h8, u32x4{ hi[0], hi[1], hi[2], hi[3] });
+            q.lo[c] = __builtin_bit_cast(h8, u32x4{ lo[0], lo[1], lo[2], lo[3] });
+        }
         return up;
     }
 }
@@ -230,16 +258,6 @@ __device__ __forceinline__ void raise(const float (&up)[NT], f32x4 (&s)[NS][NT][
     }
 }
 
-/* x - (float)half I of h, in one instruction. */
-template <int I>
-__device__ __forceinline__ float less_half(float x, uint32_t h)
-{
-    float r;
-    if constexpr (I == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
-    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
-    return r;
-}
-
 /* The weights of key tile t of a row's step, from its scores. */
 template <int TYPE, int D>
 __device__ __forceinline__ void soften(int t, f32x4 s, AttRow<D> &row, AttP<TYPE> &p)
@@ -252,13 +270,8 @@ __device__ __forceinline__ void soften(int t, f32x4 s, AttRow<D> &row, AttP<TYPE
 #pragma unroll
         for (int r = 0; r < 4; r++) p.v[r] = x[r];
     } else {
-        /* hi rounds towards zero: what it drops is in lo, to 11 more bits */
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
-            p.hi[2 * t + i] = h;
-            p.lo[2 * t + i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x[2 * i], h), less_half<1>(x[2 * i + 1], h)));
-        }
+        for (int i = 0; i < 2; i++) split(x[2 * i], x[2 * i + 1], p.hi[2 * t + i], p.lo[2 * t + i]);
     }
 }
 
@@ -363,11 +376,13 @@ __device__ __forceinline__ float *row_out(const AttnCall &a, const AttnTok &tk, 
 {
     return tk.parts == 1 ? a.out + ((size_t)t * a.heads + head) * D : a.part_o + ((size_t)(tk.part + part) * a.heads + head) * D;
 }
-/* A part's reference is +infinity where its sum is NaN, so that joining keeps it. */
+/* A part's reference is +infinity where its sum is NaN, so that joining keeps it. An empty item's parts may be
+ * more than a token has. */
 __device__ __forceinline__ void put_row(const AttnCall &a, const AttnTok &tk, int part, int t, int head, int d, int D, float ref, float l,
                                         f32x4 o, bool stats)
 {
     const bool whole = tk.parts == 1;
+    if (part >= tk.parts) return;
     *(f32x4 *)(row_out(a, tk, part, t, head, D) + d) = whole ? o * (1.0f / l) : o;
     if (!whole && stats) {
         float *ml = a.part_ml + 2 * ((size_t)(tk.part + part) * a.heads + head);
@@ -390,14 +405,21 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
     const AttnHdr &h = header(a);
-    const int n_item = h.n_work[kAttnFew] * a.kv_heads;
+    const int n_unit = h.n_run[kAttnFew] * a.kv_heads;
     const AttnWork *work = (const AttnWork *)(a.blob + h.work[kAttnFew]);
     const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
-    for (int item = blockIdx.x; item < n_item; item += gridDim.x) {
-        const AttnWork w = work[item / a.kv_heads];
-        const int kvh = item % a.kv_heads;
+    for (int u = blockIdx.x, next = -1; next >= 0 || u < n_unit;) {
+        const AttnWork w = work[next >= 0 ? next : u / a.kv_heads];
+        const int kvh = u % a.kv_heads;
+        next = w.next;
+        if (next < 0) u += gridDim.x;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
+        /* a row behind the last one takes the last one's query: its results are not stored */
+        const int qr = w.row + min(col, w.rows - 1), qt = qr / a.group;
+        AttRaw<TYPE, D> raw;
+        load_q<TYPE, D>(a.q + ((size_t)qt * a.heads + (size_t)(kvh * a.group + qr % a.group)) * D, g, raw);
+        const int limit[NT] = { min(toks[qt].pos + 1, w.key1) };
         const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
         const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
         u32x4 kf[A::NK], vf[A::NV];
@@ -431,16 +453,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
         }
         AttQ<TYPE, D> q[NT];
         AttRow<D> row[NT];
-        float up[NT], from[NT] = {};
-        int limit[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int r = w.row + 16 * n + col;
-            const bool any = 16 * n + col < w.rows;
-            const int t = any ? r / a.group : w.row / a.group;
-            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
-            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
-        }
+        float up[NT] = { make_q<TYPE, D>(raw, a.scale_log2, q[0]) }, from[NT] = {};
         const bool unit = __ballot(up[0] != 1.0f) == 0;
         for (int s = wave; s < n_step; s += kFewWaves) {
             const int key = w.key0 + s * A::KS;
@@ -535,14 +548,24 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
     const AttnHdr &h = header(a);
-    const int n_item = h.n_work[kAttnMany] * a.kv_heads;
+    const int n_unit = h.n_run[kAttnMany] * a.kv_heads;
     const AttnWork *work = (const AttnWork *)(a.blob + h.work[kAttnMany]);
     const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
-    for (int item = blockIdx.x; item < n_item; item += gridDim.x) {
-        const AttnWork w = work[item / a.kv_heads];
-        const int kvh = item % a.kv_heads;
+    for (int u = blockIdx.x, next = -1; next >= 0 || u < n_unit;) {
+        const AttnWork w = work[next >= 0 ? next : u / a.kv_heads];
+        const int kvh = u % a.kv_heads;
+        next = w.next;
+        if (next < 0) u += gridDim.x;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
+        AttRaw<TYPE, D> raw[NT];
+        int limit[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {                              /* rows behind the last one: its query, not stored */
+            const int r = w.row + min(16 * NT * wave + 16 * n + col, w.rows - 1), t = r / a.group;
+            load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, g, raw[n]);
+            limit[n] = min(toks[t].pos + 1, w.key1);
+        }
         const int n_tile = (w.key1 - w.key0 + L::KT - 1) / L::KT, last = w.key1 - 1;
         /* the next tile's pages, loaded a tile ahead of their use: in lane i the page of keys 16 (i % NG) ..,
          * and the one of the values that the thread copies */
@@ -573,7 +596,7 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
 #pragma unroll
             for (int i = 0; i < NL; i++) dma_to_lds<16>(p + i * step, vd + (i * kManyThreads + wave * 64) * 16);
         };
-        if (n_tile > 0) {                                           /* before the queries, which take as long to arrive */
+        if (n_tile > 0) {
             pages(0);
             copy(0);
             if (n_tile > 1) pages(1);
@@ -583,15 +606,8 @@ __global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_ke
         AttQ<TYPE, D> q[NT];
         AttRow<D> row[NT];
         float up[NT], from[NT] = {};
-        int limit[NT];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int i = 16 * NT * wave + 16 * n + col, r = w.row + i;
-            const bool any = i < w.rows;
-            const int t = any ? r / a.group : w.row / a.group;
-            limit[n] = any ? min(toks[t].pos + 1, w.key1) : 0;
-            up[n] = load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, any, g, a.scale_log2, q[n]);
-        }
+        for (int n = 0; n < NT; n++) up[n] = make_q<TYPE, D>(raw[n], a.scale_log2, q[n]);
         bool scaled = false;
 #pragma unroll
         for (int n = 0; n < NT; n++) scaled = scaled || up[n] != 1.0f;
@@ -843,7 +859,7 @@ __global__ __launch_bounds__(256) void attn_append_kernel(AttnAppend b)
 template <int TYPE, int D>
 hipError_t attend(const AttnCall &a, int grid, hipStream_t st)
 {
-    const int nb[kAttnKinds] = { a.live ? grid : a.h.n_work[0] * a.kv_heads, a.live ? grid : a.h.n_work[1] * a.kv_heads };
+    const int nb[kAttnKinds] = { a.live ? grid : a.h.n_run[0] * a.kv_heads, a.live ? grid : a.h.n_run[1] * a.kv_heads };
     if (nb[kAttnMany]) QLAUNCH("attend", (attn_many_kernel<TYPE, D>), dim3((unsigned)nb[kAttnMany]), dim3(kManyThreads), 0, st, a);
     if (nb[kAttnFew]) QLAUNCH("attend", (attn_few_kernel<TYPE, D>), dim3((unsigned)nb[kAttnFew]), dim3(64 * kFewWaves), 0, st, a);
     /* rows of few parts a thread group each, others kJoinLanes groups */

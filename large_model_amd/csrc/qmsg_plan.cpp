@@ -28,31 +28,40 @@ struct Segment {
     int table;              /* page table                                    */
     int pos;                /* position of the first token, -1: all see all  */
     int kind;
-    int splits, chunk;      /* items of chunk keys                           */
-    int part;               /* first of its splits among its tokens' slots   */
+    int tiles;              /* row tiles                                     */
 };
 
-int round_up(int v, int m) { return (v + m - 1) / m * m; }
+/* A segment's row tile and the items its keys are cut into. */
+struct Tile {
+    int seg, row, rows;
+    int key0, key1, full;
+    bool fresh;             /* its first item starts a run                   */
+    std::vector<int> cut;   /* where its other items start, each a run       */
+};
 
 int kind_of(int rows) { return rows <= kAttnRows[kAttnFew] ? kAttnFew : kAttnMany; }
 
-int tiles_of(const Segment &g, int G) { return (g.n_tok * G + kAttnRows[g.kind] - 1) / kAttnRows[g.kind]; }
-
-/* Blocks that fill the card, and the fewest keys worth an item of their own. */
-#ifndef FEWB
-#define FEWB 2
-#endif
-#ifndef MANYB
-#define MANYB 2
-#endif
+/* Blocks that a CU holds, the fewest keys worth a block, and what an item costs besides its keys, in keys. */
+constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };
 #ifndef FEWK
 #define FEWK 256
 #endif
 #ifndef MANYK
 #define MANYK 256
 #endif
-constexpr int kBlocksPerCu[kAttnKinds] = { FEWB, MANYB };
-constexpr int kMinKeys[kAttnKinds] = { FEWK, MANYK };
+#ifndef MANYK32
+#define MANYK32 64
+#endif
+#ifndef C0F
+#define C0F 128
+#endif
+#ifndef C0M
+#define C0M 64
+#endif
+constexpr int kMinKeys[kAttnKinds] = { FEWK, MANYK }, kMinKeysF32 = MANYK32;
+constexpr int kItemCost[kAttnKinds] = { C0F, C0M };
+/* Cuts fall on multiples of this many keys from a tile's first. */
+constexpr int kCut = 64;
 
 /* The fewest shared keys that are read once for all. */
 constexpr int kMinShared = 256;
@@ -62,9 +71,9 @@ size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
 size_t most_work(const AttnShape &s)
 {
     const size_t G = (size_t)(s.heads / s.kv_heads);
-    /* rows in a shared and an own segment, a partial tile for each segment, and the items that
-     * spreading adds: at most kBlocksPerCu blocks per CU and kind */
-    return 2 * ((size_t)s.max_tokens * G / 16) + 2 * (size_t)s.max_seq + 16384;
+    /* rows in a shared and an own segment, a partial tile for each segment; the cuts, of which each run adds
+     * one; and as many empty parts again */
+    return 2 * (2 * ((size_t)s.max_tokens * G / 16) + 2 * (size_t)s.max_seq + 16384);
 }
 
 }  // namespace
@@ -158,73 +167,167 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
             if (group) {
                 if (keys > kv_len[i] - q_len[i]) keys = kv_len[i] - q_len[i];
                 keys = keys / P * P;
-                seg.push_back({ first[(size_t)i], n_tok, 0, keys, table[(size_t)i], -1, kind_of(n_tok * G), 1, 0, 0 });
+                seg.push_back({ first[(size_t)i], n_tok, 0, keys, table[(size_t)i], -1, kind_of(n_tok * G), 0 });
             }
             for (size_t c = a; c < b; c++) {
                 const int j = used[c];
                 seg.push_back({ first[(size_t)j], q_len[j], group ? keys : 0, kv_len[j], table[(size_t)j],
-                                kv_len[j] - q_len[j], kind_of(q_len[j] * G), 1, 0, 0 });
+                                kv_len[j] - q_len[j], kind_of(q_len[j] * G), 0 });
             }
             a = b;
         }
     };
-    /* Spread each segment's keys over as many items as fill the card. */
     const size_t part_rows = attn_part_rows(s);
-    auto spread = [&](int coarser) -> bool {
-        int64_t work[kAttnKinds] = { 0, 0 };
-        for (const Segment &g : seg) work[g.kind] += (int64_t)tiles_of(g, G) * (g.key1 - g.key0) * s.kv_heads;
-        std::vector<int> parts((size_t)T, 0);
-        for (Segment &g : seg) {
-            const int64_t want = work[g.kind] / ((int64_t)kBlocksPerCu[g.kind] * n_cu) + 1;
-            const int64_t chunk = std::max<int64_t>(want, kMinKeys[g.kind]) << coarser;
-            const int64_t n = (g.key1 - g.key0 + chunk - 1) / chunk;
-            const int64_t k = std::min<int64_t>(n, coarser > 20 ? 1 : kAttnSplits);
-            g.chunk = round_up((int)((g.key1 - g.key0 + k - 1) / k), 64);
-            g.splits = (g.key1 - g.key0 + g.chunk - 1) / g.chunk;
-            g.part = parts[(size_t)g.tok];
-            for (int k = 0; k < g.n_tok; k++) parts[(size_t)(g.tok + k)] = g.part + g.splits;
+    std::vector<Tile> tiles;
+    std::vector<int> shared_parts((size_t)T), parts((size_t)T);
+    auto make_tiles = [&]() {
+        tiles.clear();
+        for (size_t i = 0; i < seg.size(); i++) {
+            Segment &g = seg[i];
+            const int R = kAttnRows[g.kind], rows = g.n_tok * G;
+            g.tiles = 0;
+            for (int r = 0; r < rows; r += R, g.tiles++) {
+                const int n = std::min(R, rows - r);
+                /* the tile's last token sees the most keys, its first the fewest */
+                const int most = g.pos < 0 ? g.key1 : g.pos + (r + n - 1) / G + 1;
+                const int least = g.pos < 0 ? g.key1 : g.pos + r / G + 1;
+                tiles.push_back({ (int)i, g.tok * G + r, n, g.key0, most, least, false, {} });
+            }
+        }
+    };
+    /* Cut the tiles' keys into runs for the blocks that the card holds. Whole tiles, longest first, where there
+     * are enough to even out (parts would cost more). Else each tile in equal pieces, a run each, where that
+     * is nearly as even as equal shares of all tiles one after the other, whose runs may span tiles and whose tiles
+     * come in more parts. `coarser`: runs that much longer, for fewer parts. */
+    auto cut_tiles = [&](int kind, int64_t coarser) {
+        std::vector<Tile *> of;
+        int64_t cost = 0;
+        for (Tile &x : tiles)
+            if (seg[(size_t)x.seg].kind == kind) {
+                of.push_back(&x);
+                x.cut.clear();
+                x.fresh = true;
+                cost += x.key1 - x.key0 + kItemCost[kind];
+            }
+        const int64_t slots = std::max<int64_t>(1, (int64_t)kBlocksPerCu[kind] * n_cu / s.kv_heads);
+        if (of.empty() || (int64_t)of.size() >= 2 * slots) return;
+        const int64_t floor = kind == kAttnMany && s.type == 0 ? kMinKeysF32 : kMinKeys[kind];
+        /* the shortest pieces of which there are no more than slots */
+        int64_t piece = std::max((cost / slots + kCut - 1) / kCut * kCut, floor) * coarser, n_run = slots + 1;
+        for (; (int64_t)of.size() <= slots; piece += piece / 64 / kCut * kCut + kCut) {
+            n_run = 0;
+            for (const Tile *x : of) n_run += (x->key1 - x->key0 + piece - 1) / piece;
+            if (n_run <= slots) break;
+        }
+        int64_t share = std::max(cost / slots, floor) * coarser + kItemCost[kind];
+        if (n_run <= slots && piece + kItemCost[kind] <= share + share / 8) {
+            for (Tile *x : of) {
+                const int64_t len = x->key1 - x->key0, n = (len + piece - 1) / piece, each = ((len + n - 1) / n + kCut - 1) / kCut * kCut;
+                for (int64_t at = each; at < len; at += each) x->cut.push_back(x->key0 + (int)at);
+            }
+            return;
+        }
+        for (n_run = slots + 1; n_run > slots; share += share / 64 + kCut) {
+            int64_t room = 0;
+            n_run = 0;
+            for (Tile *x : of) {
+                x->cut.clear();
+                x->fresh = false;
+                for (int at = x->key0;;) {
+                    /* no sliver at the end of a run, nor (an eighth over) of a tile */
+                    if (room < kItemCost[kind] + std::min<int64_t>(share / 8, 2 * kCut)) {
+                        room = share;
+                        n_run++;
+                        if (at == x->key0) x->fresh = true;
+                        else x->cut.push_back(at);
+                    }
+                    const int64_t left = x->key1 - at + kItemCost[kind], take = (room - kItemCost[kind] + kCut - 1) / kCut * kCut;
+                    if (left <= room + share / 8 || at + take >= x->key1) {
+                        room -= left;
+                        break;
+                    }
+                    at += (int)take;
+                    room = 0;
+                }
+            }
+        }
+    };
+    /* Parts of every token: those of the shared segment (as many for all of its tokens), then the most
+     * that a tile of the token's own segment is cut into. */
+    auto count_parts = [&]() -> bool {
+        std::fill(shared_parts.begin(), shared_parts.end(), 0);
+        std::fill(parts.begin(), parts.end(), 0);
+        size_t x = 0;
+        for (const Segment &g : seg) {
+            int most = 0;
+            for (int k = 0; k < g.tiles; k++) most = std::max(most, (int)tiles[x + (size_t)k].cut.size() + 1);
+            for (int k = 0; k < g.tiles; k++, x++) {
+                const Tile &y = tiles[x];
+                for (int q = y.row / G; q <= (y.row + y.rows - 1) / G; q++) {
+                    if (g.pos < 0) shared_parts[(size_t)q] = most;
+                    else parts[(size_t)q] = std::max(parts[(size_t)q], (int)y.cut.size() + 1);
+                }
+            }
         }
         size_t slots = 0;
         for (int k = 0; k < (int)T; k++) {
-            tok[(size_t)k].parts = parts[(size_t)k];
+            tok[(size_t)k].parts = shared_parts[(size_t)k] + parts[(size_t)k];
             tok[(size_t)k].part = (int32_t)slots;
-            if (parts[(size_t)k] > 1) slots += (size_t)parts[(size_t)k];
+            if (tok[(size_t)k].parts > 1) slots += (size_t)tok[(size_t)k].parts;
         }
         return slots * (size_t)s.heads <= part_rows;
     };
-    /* a segment follows the shared one of its tokens, so its slots come after that one's */
     bool fits = false;
     for (int share = 1; share >= 0 && !fits; share--) {
         segments(share != 0);
-        for (int coarser = 0; coarser <= 21 && !fits; coarser++) fits = spread(coarser);
+        make_tiles();
+        for (int64_t coarser = 1; coarser <= (int64_t)1 << 32 && !fits; coarser *= 2) {
+            for (int k = 0; k < kAttnKinds; k++) cut_tiles(k, coarser);
+            fits = count_parts();
+        }
     }
 
     std::vector<AttnWork> work[kAttnKinds];
-    for (const Segment &g : seg) {
-        const int R = kAttnRows[g.kind], rows = g.n_tok * G;
-        for (int r = 0; r < rows; r += R) {
-            const int n = std::min(R, rows - r);
-            /* the tile's last token sees the most keys, its first the fewest */
-            const int most = g.pos < 0 ? g.key1 : g.pos + (r + n - 1) / G + 1;
-            const int least = g.pos < 0 ? g.key1 : g.pos + r / G + 1;
-            for (int k = 0; k < g.splits; k++) {
-                const int64_t k0 = (int64_t)g.key0 + (int64_t)k * g.chunk;
+    int n_run[kAttnKinds];
+    for (int kind = 0; kind < kAttnKinds; kind++) {
+        std::vector<AttnWork> &first = work[kind], later, empty;
+        std::vector<int> run;                                  /* of each later item */
+        for (const Tile &x : tiles) {
+            const Segment &g = seg[(size_t)x.seg];
+            if (g.kind != kind) continue;
+            int need = 0;           /* a token in two tiles has the parts of the one that is cut more */
+            for (int q = x.row / G; q <= (x.row + x.rows - 1) / G; q++)
+                need = std::max(need, g.pos < 0 ? shared_parts[(size_t)q] : parts[(size_t)q]);
+            const int base = g.pos < 0 ? 0 : shared_parts[(size_t)(x.row / G)], n = (int)x.cut.size() + 1;
+            for (int k = 0; k < need; k++) {
                 AttnWork w{};
-                w.row = g.tok * G + r;
-                w.rows = n;
+                w.row = x.row;
+                w.rows = x.rows;
                 w.pages = g.table;
-                w.key0 = (int)std::min<int64_t>(k0, g.key1 / 16 * 16);
-                w.key1 = (int)std::min<int64_t>(k0 + g.chunk, most);
-                if (w.key1 < w.key0 || k0 >= most) w.key1 = w.key0;        /* no keys: an empty part */
-                w.full = std::min(least, w.key1);
-                w.part = g.part + k;
-                work[g.kind].push_back(w);
+                w.key0 = k && k < n ? x.cut[(size_t)k - 1] : x.key0;
+                w.key1 = k >= n ? w.key0 : k + 1 < n ? x.cut[(size_t)k] : x.key1;
+                w.full = std::min(x.full, w.key1);
+                w.part = base + k;
+                w.next = -1;
+                if (k >= n) empty.push_back(w);
+                else if (k || x.fresh) first.push_back(w);
+                else {
+                    later.push_back(w);
+                    run.push_back((int)first.size() - 1);
+                }
             }
         }
+        /* runs of an item each start with the longest: the last ones end soon after another */
+        if (later.empty()) std::stable_sort(first.begin(), first.end(), [](const AttnWork &a, const AttnWork &b) { return a.key1 - a.key0 > b.key1 - b.key0; });
+        first.insert(first.end(), empty.begin(), empty.end());
+        n_run[kind] = (int)first.size();
+        for (size_t i = later.size(); i-- > 0;) {              /* a run's items after its first, in their order */
+            AttnWork &head = first[(size_t)run[i]];
+            later[i].next = head.next;
+            head.next = n_run[kind] + (int)i;
+        }
+        first.insert(first.end(), later.begin(), later.end());
     }
-    /* longest items first: the last ones to start end soon */
-    for (auto &w : work)
-        std::stable_sort(w.begin(), w.end(), [](const AttnWork &a, const AttnWork &b) { return a.key1 - a.key0 > b.key1 - b.key0; });
 
     std::vector<int32_t> comb;
     for (int k = 0; k < (int)T; k++)
@@ -245,7 +348,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     h.vt = place(vt.size() * sizeof(AttnVTile));
     h.comb = place(comb.size() * 4);
     for (int k = 0; k < kAttnKinds; k++) {
-        h.n_work[k] = (int)work[k].size();
+        h.n_run[k] = n_run[k];
         h.work[k] = place(work[k].size() * sizeof(AttnWork));
     }
     h.pages = place(ids.size() * 4);

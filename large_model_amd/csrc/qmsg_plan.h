@@ -2,9 +2,10 @@
  * the HIP runtime: qmsg_attn_batch checks a batch and plans it here, the kernels read the result.
  *
  * Rows are (token, query head of the kv head's group), token-major: row t * G + g. A work item is a
- * tile of rows against a range of keys of one page table, for every kv head. Rows whose keys are
- * spread over several items leave partial results (reference maximum, sum, weighted values) in
- * slots of their own, which the combine kernel joins in slot order. */
+ * tile of rows against a range of keys of one page table, for every kv head; a run is the items
+ * that one block works through. Rows whose keys are spread over several items leave partial
+ * results (reference maximum, sum, weighted values) in slots of their own, which the join kernel
+ * takes together in slot order. */
 #ifndef QMSG_PLAN_H
 #define QMSG_PLAN_H
 
@@ -21,7 +22,7 @@ struct AttnTok {
     int32_t pos;      /* position in its sequence: it sees keys 0 .. pos */
     int32_t dst;      /* page * page_tokens + slot of its key and value   */
     int32_t part;     /* first partial slot, where parts > 1              */
-    int32_t parts;    /* items its keys are spread over                   */
+    int32_t parts;    /* items its keys are spread over (a tile's: at most) */
 };
 
 /* Up to kVTile tokens whose values go to neighbouring slots of one page. */
@@ -36,20 +37,18 @@ struct AttnWork {
     int32_t key0, key1;     /* keys of this item (key0 a multiple of 16)                  */
     int32_t full;           /* every row sees the keys below this one                     */
     int32_t part;           /* which of its rows' partial slots it fills                  */
-    int32_t pad;
+    int32_t next;           /* the run's next item, or -1                                 */
 };
 
 /* Row tiles of the kernels: waves that split the keys, waves that split the rows and share the keys
  * through LDS. */
 enum { kAttnFew = 0, kAttnMany = 1, kAttnKinds = 2 };
 constexpr int kAttnRows[kAttnKinds] = { 16, 128 };
-/* A segment's keys are spread over at most this many items. */
-constexpr int kAttnSplits = 64;
-
 /* Where the parts of a batch sit in its blob (byte offsets) and how many there are. */
 struct AttnHdr {
-    int32_t n_tok, n_vt, n_comb, max_parts, n_work[kAttnKinds];
+    int32_t n_tok, n_vt, n_comb, max_parts, n_run[kAttnKinds];
     int32_t tok, vt, comb, work[kAttnKinds], pages, bytes;
+    /* run r of a kind starts with item r */
 };
 
 struct AttnShape {
@@ -61,7 +60,7 @@ struct AttnShape {
 constexpr size_t kAttnPartRows = (size_t)1 << 18;
 inline size_t attn_part_rows(const AttnShape &s)
 {
-    const size_t most = (size_t)s.max_tokens * (size_t)s.heads * 2 * kAttnSplits;
+    const size_t most = (size_t)s.max_tokens * (size_t)s.heads * 128;
     return most < kAttnPartRows ? most : kAttnPartRows;
 }
 /* Bytes that hold any batch of this shape. */

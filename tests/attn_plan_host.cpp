@@ -66,7 +66,15 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
     std::map<int, std::vector<std::pair<int, int>>> ranges;
     for (int kind = 0; kind < kAttnKinds; kind++) {
         const AttnWork *w = (const AttnWork *)(p.blob.data() + h.work[kind]);
-        for (int i = 0; i < h.n_work[kind]; i++) {
+        const int n_item = ((kind + 1 < kAttnKinds ? h.work[kind + 1] : h.pages) - h.work[kind]) / (int)sizeof(AttnWork);
+        std::vector<int> reached;
+        for (int r = 0; r < h.n_run[kind]; r++)
+            for (int i = r; i >= 0; i = w[i].next) {
+                CHECK(i < n_item && (i == r) == (i < h.n_run[kind]) && (int)reached.size() < n_item);
+                reached.push_back(i);
+            }
+        CHECK((int)reached.size() == n_item);
+        for (int i : reached) {
             CHECK(w[i].rows > 0 && w[i].rows <= kAttnRows[kind] && w[i].row >= 0 && w[i].row + w[i].rows <= T * G);
             CHECK(w[i].key0 >= 0 && w[i].key0 % 16 == 0 && w[i].key1 >= w[i].key0 && w[i].full <= w[i].key1);
             CHECK(w[i].key1 == w[i].key0 || w[i].pages + (w[i].key1 - 1) / P < n_ids);
@@ -74,7 +82,10 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
             if (s0 != s1) *shared = true;
             for (int r = w[i].row; r < w[i].row + w[i].rows; r++) {
                 const int t = r / G, sq = seq[(size_t)t], lim = std::min(tok[t].pos + 1, w[i].key1);
-                CHECK(w[i].part >= 0 && w[i].part < tok[t].parts && parts.insert({ r, w[i].part }).second);
+                /* a row of a token that another tile gives fewer parts leaves an empty item's */
+                CHECK(w[i].part >= 0 && (w[i].part < tok[t].parts || w[i].key1 == w[i].key0));
+                if (w[i].part >= tok[t].parts) continue;
+                CHECK(parts.insert({ r, w[i].part }).second);
                 CHECK(w[i].full <= tok[t].pos + 1);
                 if (lim <= w[i].key0) continue;
                 ranges[r].push_back({ w[i].key0, lim });
