@@ -32,6 +32,7 @@ namespace qmsg {
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLowest = -INFINITY;
 
@@ -109,11 +110,12 @@ __device__ __forceinline__ float less_half(float x, uint32_t h)
     return r;
 }
 
-/* x and y as two f16 each. hi rounds towards zero: what it drops is in lo, to 11 more bits. */
+/* x and y as two f16 each: what hi's 11 bits leave out is in lo, to 11 more. */
 __device__ __forceinline__ void split(float x, float y, uint32_t &hi, uint32_t &lo)
 {
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x, hi), less_half<1>(y, hi)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{ x, y }), h2));
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{ less_half<0>(x, hi), less_half<1>(y, hi) }), h2));
 }
 
 /* A query times `scale` as B operand; returns the power of two that its scores come out multiplied with: 1
@@ -526,8 +528,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 /* Many rows (128): four waves of 32 rows each share tiles of keys and values, copied to LDS by the LDS
  * DMA, the next tile's copy in flight while one is worked on. Pieces are stored with their index in
  * the row xored by the row, so that the 16 rows a wave instruction reads lie in all banks. */
-constexpr int kManyNT = 2;
-constexpr int kManyThreads = 64 * 128 / (16 * kManyNT);
+constexpr int kManyThreads = 256;
 
 template <int TYPE, int D>
 struct ManyLds {
@@ -536,11 +537,11 @@ struct ManyLds {
 };
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kManyThreads, kManyThreads / 128) void attn_many_kernel(AttnCall a)
+__global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
 {
     using A = Att<TYPE, D>;
     using L = ManyLds<TYPE, D>;
-    constexpr int NT = kManyNT, RC = D / A::CE, VC = L::KT / A::CE, NG = L::KT / 16;
+    constexpr int NT = attn_rows(kAttnMany, TYPE) / 64, RC = D / A::CE, VC = L::KT / A::CE, NG = L::KT / 16;
     constexpr int NL = L::BYTES / 16 / kManyThreads;                /* pieces per thread          */
     constexpr int RP = D * A::ES >= 256 ? 1 : 256 / (D * A::ES);    /* key rows per 256 bytes     */
     static_assert(VC == 8, "a row of values is 128 bytes");

@@ -39,7 +39,7 @@ struct Tile {
     std::vector<int> cut;   /* where its other items start, each a run       */
 };
 
-int kind_of(int rows) { return rows <= kAttnRows[kAttnFew] ? kAttnFew : kAttnMany; }
+int kind_of(int rows) { return rows <= attn_rows(kAttnFew, 1) ? kAttnFew : kAttnMany; }
 
 /* Blocks that a CU holds, the fewest keys worth a block, and what an item costs besides its keys, in keys. */
 constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };
@@ -50,7 +50,7 @@ constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };
 #define MANYK 256
 #endif
 #ifndef MANYK32
-#define MANYK32 64
+#define MANYK32 128
 #endif
 #ifndef C0F
 #define C0F 128
@@ -184,7 +184,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
         tiles.clear();
         for (size_t i = 0; i < seg.size(); i++) {
             Segment &g = seg[i];
-            const int R = kAttnRows[g.kind], rows = g.n_tok * G;
+            const int R = attn_rows(g.kind, s.type), rows = g.n_tok * G;
             g.tiles = 0;
             for (int r = 0; r < rows; r += R, g.tiles++) {
                 const int n = std::min(R, rows - r);

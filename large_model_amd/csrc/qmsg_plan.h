@@ -43,7 +43,7 @@ struct AttnWork {
 /* Row tiles of the kernels: waves that split the keys, waves that split the rows and share the keys
  * through LDS. */
 enum { kAttnFew = 0, kAttnMany = 1, kAttnKinds = 2 };
-constexpr int kAttnRows[kAttnKinds] = { 16, 128 };
+constexpr int attn_rows(int kind, int type) { return kind == kAttnFew ? 16 : type == 0 ? 64 : 128; }
 /* Where the parts of a batch sit in its blob (byte offsets) and how many there are. */
 struct AttnHdr {
     int32_t n_tok, n_vt, n_comb, max_parts, n_run[kAttnKinds];

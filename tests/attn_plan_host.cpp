@@ -75,7 +75,7 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
             }
         CHECK((int)reached.size() == n_item);
         for (int i : reached) {
-            CHECK(w[i].rows > 0 && w[i].rows <= kAttnRows[kind] && w[i].row >= 0 && w[i].row + w[i].rows <= T * G);
+            CHECK(w[i].rows > 0 && w[i].rows <= attn_rows(kind, s.type) && w[i].row >= 0 && w[i].row + w[i].rows <= T * G);
             CHECK(w[i].key0 >= 0 && w[i].key0 % 16 == 0 && w[i].key1 >= w[i].key0 && w[i].full <= w[i].key1);
             CHECK(w[i].key1 == w[i].key0 || w[i].pages + (w[i].key1 - 1) / P < n_ids);
             const int s0 = seq[(size_t)(w[i].row / G)], s1 = seq[(size_t)((w[i].row + w[i].rows - 1) / G)];
@@ -116,7 +116,7 @@ int main(int argc, char **argv)
     for (batch = 0; batch < atoi(argc > 2 ? argv[2] : "1"); batch++) {
         static const int kHeads[][2] = { { 1, 1 }, { 14, 2 }, { 16, 16 }, { 32, 4 }, { 64, 4 }, { 6, 2 } };
         const int *hd = kHeads[pick(0, 5)];
-        AttnShape s{ hd[0], hd[1], 128, 1, 16 << pick(0, 4), 0, pick(1, 24), 0, 0 };
+        AttnShape s{ hd[0], hd[1], 128, pick(0, 1), 16 << pick(0, 4), 0, pick(1, 24), 0, 0 };
         const int n_seq = pick(0, s.max_seq), mode = pick(0, 3), most = pick(0, 1) ? 40 : 5000;
         std::vector<int> q, kv;
         const int shared = mode == 3 ? pick(0, most / s.page) : 0;
