@@ -22,6 +22,7 @@ struct AttnCall {
     float scale_log2;           /* scale * log2(e)                 */
     const float *q;             /* [T][heads][D]                   */
     float *out;                 /* [T][heads][D]                   */
+    int32_t *done;              /* counters, 0 between calls       */
     float *part_o, *part_ml;    /* partial rows [slot][heads][D], their reference and sum [slot][heads][2] */
 };
 

@@ -33,6 +33,7 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLowest = -INFINITY;
 
@@ -373,6 +374,23 @@ __device__ __forceinline__ f32x4 wild_sum(const uint8_t *pool, const int32_t *ta
 /* The part of a call's header that is in use: the launch's own, or the blob's for a captured call. */
 __device__ __forceinline__ const AttnHdr &header(const AttnCall &a) { return a.live ? *(const AttnHdr *)a.blob : a.h; }
 
+/* Parts that a block joins go past its die's L2 (and are read past it): it may run on another than theirs. A
+ * release and an acquire of the whole L2 instead took 262 us where this takes 55 (32 decoded sequences). */
+__device__ __forceinline__ void put_far(float *p, f32x4 v)
+{
+    const uint64_t x = __builtin_bit_cast(uint64_t, (f32x2){ v.x, v.y }), y = __builtin_bit_cast(uint64_t, (f32x2){ v.z, v.w });
+    __hip_atomic_store((uint64_t *)p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((uint64_t *)p + 1, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put_far(float *p, float a, float b)
+{
+    __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, (f32x2){ a, b }), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 get_far(const float *p)
+{
+    return __builtin_bit_cast(f32x2, __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
 /* Where a row's results go: the output where the token has no other part, else its part. */
 __device__ __forceinline__ float *row_out(const AttnCall &a, const AttnTok &tk, int part, int t, int head, int D)
 {
@@ -380,16 +398,73 @@ __device__ __forceinline__ float *row_out(const AttnCall &a, const AttnTok &tk, 
 }
 /* A part's reference is +infinity where its sum is NaN, so that joining keeps it. An empty item's parts may be
  * more than a token has. */
-__device__ __forceinline__ void put_row(const AttnCall &a, const AttnTok &tk, int part, int t, int head, int d, int D, float ref, float l,
-                                        f32x4 o, bool stats)
+__device__ __forceinline__ void put_row(const AttnCall &a, const AttnTok &tk, const AttnWork &w, int t, int head, int d, int D, float ref,
+                                        float l, f32x4 o, bool stats)
 {
     const bool whole = tk.parts == 1;
-    if (part >= tk.parts) return;
-    *(f32x4 *)(row_out(a, tk, part, t, head, D) + d) = whole ? o * (1.0f / l) : o;
-    if (!whole && stats) {
-        float *ml = a.part_ml + 2 * ((size_t)(tk.part + part) * a.heads + head);
-        ml[0] = l != l ? INFINITY : ref;
-        ml[1] = l;
+    if (w.part >= tk.parts) return;
+    float *to = row_out(a, tk, w.part, t, head, D) + d, *ml = a.part_ml + 2 * ((size_t)(tk.part + w.part) * a.heads + head);
+    ref = l != l ? INFINITY : ref;
+    if (whole) {
+        *(f32x4 *)to = o * (1.0f / l);
+    } else if (w.count >= 0) {
+        put_far(to, o);
+        if (stats) put_far(ml, ref, l);
+    } else {
+        *(f32x4 *)to = o;
+        if (stats) *(f32x2 *)ml = f32x2{ ref, l };
+    }
+}
+
+/* Parts of four values taken together: o = sum_p 2^(m_p - m) o_p, l likewise. */
+struct AttJoin {
+    float m = kLowest, l = 0.0f;
+    f32x4 o = { 0, 0, 0, 0 };
+    __device__ __forceinline__ void add(float mp, float lp, f32x4 op)
+    {
+        if (mp == kLowest) return;                                  /* saw no key */
+        const float top = fmaxf(m, mp), f0 = m == kLowest ? 0.0f : exp2_fast(m - top), f1 = exp2_fast(mp - top);
+        m = top;
+        l = l * f0 + lp * f1;
+        o = o * f0 + op * f1;
+    }
+};
+
+/* After an item of a tile whose parts its last item joins: count it, and join if it is the last. Each wave waits
+ * until its parts have arrived before the block counts. */
+template <int D, int THREADS>
+__device__ __forceinline__ void join_tile(const AttnCall &a, const AttnTok *toks, const AttnWork &w, int kvh, int &s_last)
+{
+    if (w.count < 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int32_t *c = a.done + w.count * a.kv_heads + kvh;
+        s_last = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == w.joins - 1;
+        if (s_last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    for (int e = threadIdx.x; e < w.rows * (D / 4); e += THREADS) {
+        const int r = w.row + e / (D / 4), d = e % (D / 4) * 4, t = r / a.group, head = kvh * a.group + r % a.group;
+        const AttnTok tk = toks[t];
+        if (tk.parts == 1) continue;                                /* is in the output */
+        const size_t r0 = (size_t)tk.part * a.heads + head;
+        AttJoin j;
+        for (int p = 0; p < tk.parts; p += 4) {                     /* four parts' loads at a time */
+            f32x2 ml[4], lo[4], hi[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const size_t at = r0 + (size_t)min(p + k, tk.parts - 1) * a.heads;
+                ml[k] = get_far(a.part_ml + 2 * at);
+                lo[k] = get_far(a.part_o + at * D + d);
+                hi[k] = get_far(a.part_o + at * D + d + 2);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (p + k < tk.parts) j.add(ml[k].x, ml[k].y, f32x4{ lo[k].x, lo[k].y, hi[k].x, hi[k].y });
+        }
+        *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + d) = j.o * (1.0f / j.l);
     }
 }
 
@@ -404,6 +479,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
     constexpr int NT = 1;
     __shared__ __align__(16) float s_o[kFewWaves][16][D + 4];
     __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16];
+    __shared__ int s_last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
     const AttnHdr &h = header(a);
@@ -518,10 +594,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
                 const int r = w.row + 16 * n + rr, t = r / a.group;
                 if (__builtin_expect(wild, 0))
                     o += wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, min(toks[t].pos + 1, w.key1), d);
-                put_row(a, toks[t], w.part, t, kvh * a.group + r % a.group, d, D, mm, ll, o, d == 0);
+                put_row(a, toks[t], w, t, kvh * a.group + r % a.group, d, D, mm, ll, o, d == 0);
             }
             __syncthreads();
         }
+        join_tile<D, 64 * kFewWaves>(a, toks, w, kvh, s_last);
     }
 }
 
@@ -700,7 +777,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
             const AttnTok tk = toks[t];
 #pragma unroll
             for (int k = 0; k < D / 16; k++)
-                put_row(a, tk, w.part, t, head, 16 * k + 4 * g, D, row[n].ref, l, row[n].o[k], k == 0 && g == 0);
+                put_row(a, tk, w, t, head, 16 * k + 4 * g, D, row[n].ref, l, row[n].o[k], k == 0 && g == 0);
             if (__builtin_expect(__ballot(bad) != 0, 0)) {
                 float *o = row_out(a, tk, w.part, t, head, D);
 #pragma unroll 1
@@ -732,35 +809,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
         const int i = min(i0 + rb, n - 1), t = comb[i / a.heads], head = i % a.heads;
         const AttnTok tk = toks[t];
         const size_t r0 = (size_t)tk.part * a.heads + head;
-        float m = kLowest, l = 0.0f;
-        f32x4 o = { 0, 0, 0, 0 };
-        auto add = [&](float mp, float lp, f32x4 op) {
-            if (mp == kLowest) return;                              /* saw no key */
-            const float top = fmaxf(m, mp), f0 = m == kLowest ? 0.0f : exp2_fast(m - top), f1 = exp2_fast(mp - top);
-            m = top;
-            l = l * f0 + lp * f1;
-            o = o * f0 + op * f1;
-        };
+        AttJoin j;
         /* two parts' loads at a time */
         for (int p = pl; p < tk.parts; p += 2 * PL) {
             const size_t r = r0 + (size_t)p * a.heads, r2 = p + PL < tk.parts ? r + (size_t)PL * a.heads : r;
             const float m1 = a.part_ml[2 * r], l1 = a.part_ml[2 * r + 1], m2 = a.part_ml[2 * r2], l2 = a.part_ml[2 * r2 + 1];
             const f32x4 o1 = *(const f32x4 *)(a.part_o + r * D + 4 * d), o2 = *(const f32x4 *)(a.part_o + r2 * D + 4 * d);
-            add(m1, l1, o1);
-            if (r2 != r) add(m2, l2, o2);
+            j.add(m1, l1, o1);
+            if (r2 != r) j.add(m2, l2, o2);
         }
         if constexpr (PL > 1) {
-            s_o[pl][rb][d] = o;
+            s_o[pl][rb][d] = j.o;
             if (d == 0) {
-                s_m[pl][rb] = m;
-                s_l[pl][rb] = l;
+                s_m[pl][rb] = j.m;
+                s_l[pl][rb] = j.l;
             }
             __syncthreads();
             if (pl == 0)
-                for (int k = 1; k < PL; k++) add(s_m[k][rb], s_l[k][rb], s_o[k][rb][d]);
+                for (int k = 1; k < PL; k++) j.add(s_m[k][rb], s_l[k][rb], s_o[k][rb][d]);
             __syncthreads();
         }
-        if (pl == 0 && i0 + rb < n) *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + 4 * d) = o * (1.0f / l);
+        if (pl == 0 && i0 + rb < n) *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + 4 * d) = j.o * (1.0f / j.l);
     }
 }
 

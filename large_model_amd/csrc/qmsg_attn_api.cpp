@@ -90,6 +90,7 @@ int make_call(qmsg_ctx *c, const AttnStore &a, int layer, AttnCall *o)
     k.kv_heads = a.cfg.n_head_kv;
     k.group = a.cfg.n_head / a.cfg.n_head_kv;
     k.scale_log2 = (float)((a.cfg.scale > 0.0f ? (double)a.cfg.scale : 1.0 / std::sqrt((double)a.cfg.head_dim)) * 1.4426950408889634);
+    k.done = a.done;
     k.part_o = a.part_o;
     k.part_ml = a.part_ml;
     *o = k;
@@ -151,8 +152,10 @@ static int attn_new(qmsg_ctx *c, const qmsg_attn_cfg &f, void *d_k, void *d_v, A
     const int n = f.head_dim / 2;
     if ((rc = dev_alloc(c, (void **)&a.freq, (size_t)n * 8, a.allocs)) || (rc = dev_alloc(c, (void **)&a.blob, blob, a.allocs)) ||
         (rc = dev_alloc(c, (void **)&a.part_o, rows * (size_t)f.head_dim * 4, a.allocs)) ||
-        (rc = dev_alloc(c, (void **)&a.part_ml, rows * 8, a.allocs)))
+        (rc = dev_alloc(c, (void **)&a.part_ml, rows * 8, a.allocs)) ||
+        (rc = dev_alloc(c, (void **)&a.done, kAttnCounters * 4, a.allocs)))
         return rc;
+    HIP_TRY(c, hipMemset(a.done, 0, kAttnCounters * 4));
     double freq[64];
     for (int i = 0; i < n; i++) freq[i] = std::pow((double)f.rope_base, -(double)i / n) / 6.283185307179586476925;
     HIP_TRY(c, hipMemcpy(a.freq, freq, (size_t)n * 8, hipMemcpyHostToDevice));

@@ -52,6 +52,7 @@ struct AttnStore {
     double *freq = nullptr;                 /* [D/2] turns per position                */
     uint8_t *blob = nullptr;                /* the batch's plan on the device          */
     float *part_o = nullptr, *part_ml = nullptr;
+    int32_t *done = nullptr;                /* counters of the tiles' done items       */
     AttnPlan plan;
     /* two pinned plans: one is filled while the copy of the other may still run */
     uint8_t *pin[2] = { nullptr, nullptr };

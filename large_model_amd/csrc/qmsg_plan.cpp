@@ -47,7 +47,7 @@ constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };
 #define FEWK 256
 #endif
 #ifndef MANYK
-#define MANYK 256
+#define MANYK 384
 #endif
 #ifndef MANYK32
 #define MANYK32 128
@@ -288,7 +288,8 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     }
 
     std::vector<AttnWork> work[kAttnKinds];
-    int n_run[kAttnKinds];
+    int n_run[kAttnKinds], counters = 0;
+    std::vector<char> apart((size_t)T, 0);                    /* tokens that the join kernel takes */
     for (int kind = 0; kind < kAttnKinds; kind++) {
         std::vector<AttnWork> &first = work[kind], later, empty;
         std::vector<int> run;                                  /* of each later item */
@@ -299,6 +300,10 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
             for (int q = x.row / G; q <= (x.row + x.rows - 1) / G; q++)
                 need = std::max(need, g.pos < 0 ? shared_parts[(size_t)q] : parts[(size_t)q]);
             const int base = g.pos < 0 ? 0 : shared_parts[(size_t)(x.row / G)], n = (int)x.cut.size() + 1;
+            /* a tile whose rows have no parts but its own items' */
+            const bool own = kind == kAttnFew && need > 1 && need <= kAttnJoins && g.pos >= 0 && base == 0 && (counters + 1) * s.kv_heads <= kAttnCounters;
+            const int count = own ? counters++ : -1;
+            for (int q = x.row / G; q <= (x.row + x.rows - 1) / G; q++) apart[(size_t)q] |= !own;
             for (int k = 0; k < need; k++) {
                 AttnWork w{};
                 w.row = x.row;
@@ -309,6 +314,8 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
                 w.full = std::min(x.full, w.key1);
                 w.part = base + k;
                 w.next = -1;
+                w.joins = need;
+                w.count = count;
                 if (k >= n) empty.push_back(w);
                 else if (k || x.fresh) first.push_back(w);
                 else {
@@ -331,7 +338,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
 
     std::vector<int32_t> comb;
     for (int k = 0; k < (int)T; k++)
-        if (tok[(size_t)k].parts > 1) comb.push_back(k);
+        if (tok[(size_t)k].parts > 1 && apart[(size_t)k]) comb.push_back(k);
 
     AttnHdr h{};
     size_t at = align16(sizeof(AttnHdr));

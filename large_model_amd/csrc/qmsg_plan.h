@@ -38,6 +38,9 @@ struct AttnWork {
     int32_t full;           /* every row sees the keys below this one                     */
     int32_t part;           /* which of its rows' partial slots it fills                  */
     int32_t next;           /* the run's next item, or -1                                 */
+    int32_t joins, count;   /* items of the tile, and the counter of those that are done (the
+                             * last one joins the tile's parts), or -1: the join kernel does  */
+    int32_t pad[2];
 };
 
 /* Row tiles of the kernels: waves that split the keys, waves that split the rows and share the keys
@@ -63,6 +66,12 @@ inline size_t attn_part_rows(const AttnShape &s)
     const size_t most = (size_t)s.max_tokens * (size_t)s.heads * 128;
     return most < kAttnPartRows ? most : kAttnPartRows;
 }
+/* Few rows' tiles of up to this many items are joined by the last of them, which saves a launch (us of a token
+ * over 513 keys in three items 4.1 / 7.3, alone 22 / 27); its block reads what the join kernel spreads over
+ * the card, which took 64 / 42 us alone for tiles of 80 rows in 16 items (kAttnMany, left to that kernel). */
+constexpr int kAttnJoins = 16;
+/* Counters of done items (a tile's, for each kv head). */
+constexpr int kAttnCounters = 1 << 14;
 /* Bytes that hold any batch of this shape. */
 size_t attn_blob_bytes(const AttnShape &s);
 

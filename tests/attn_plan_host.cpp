@@ -52,15 +52,19 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
     for (int v : seen) CHECK(v == 1);
     /* parts: ranges of their own, as many as the workspace has */
     size_t slots = 0;
-    int n_comb = 0;
+    std::set<int> apart(comb, comb + h.n_comb);
+    CHECK((int)apart.size() == h.n_comb);
     for (int t = 0; t < T; t++) {
         CHECK(tok[t].parts >= 1);
         if (tok[t].parts == 1) continue;
-        CHECK(tok[t].part == (int)slots && comb[n_comb] == t);
+        CHECK(tok[t].part == (int)slots);
         slots += (size_t)tok[t].parts;
-        n_comb++;
     }
-    CHECK(n_comb == h.n_comb && slots * (size_t)s.heads <= attn_part_rows(s));
+    CHECK(slots * (size_t)s.heads <= attn_part_rows(s));
+    /* rows of several parts are joined: by the join kernel, or by the last of their tile's items, which
+     * leaves all of them */
+    std::map<int, std::vector<int>> counted;
+    std::set<int> joined;
     /* items: (row, part) once; the keys of a row's items are 0 .. pos, each once, on its own pages */
     std::set<std::pair<int, int>> parts;
     std::map<int, std::vector<std::pair<int, int>>> ranges;
@@ -78,6 +82,20 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
             CHECK(w[i].rows > 0 && w[i].rows <= attn_rows(kind, s.type) && w[i].row >= 0 && w[i].row + w[i].rows <= T * G);
             CHECK(w[i].key0 >= 0 && w[i].key0 % 16 == 0 && w[i].key1 >= w[i].key0 && w[i].full <= w[i].key1);
             CHECK(w[i].key1 == w[i].key0 || w[i].pages + (w[i].key1 - 1) / P < n_ids);
+            if (w[i].count >= 0) {
+                CHECK((w[i].count + 1) * s.kv_heads <= kAttnCounters && w[i].joins <= kAttnJoins);
+                auto &v = counted[w[i].count];
+                v.push_back(w[i].part);
+                if (v.size() == 1) v.push_back(w[i].row);
+                CHECK(v[1] == w[i].row && (int)v.size() <= w[i].joins + 1);
+                if ((int)v.size() == w[i].joins + 1)
+                    for (int r = w[i].row; r < w[i].row + w[i].rows; r++) {
+                        CHECK(tok[r / G].parts <= w[i].joins && joined.insert(r).second);
+                        std::set<int> all(v.begin() + 2, v.end());
+                        all.insert(v[0]);
+                        for (int k = 0; k < tok[r / G].parts; k++) CHECK(all.count(k));
+                    }
+            }
             const int s0 = seq[(size_t)(w[i].row / G)], s1 = seq[(size_t)((w[i].row + w[i].rows - 1) / G)];
             if (s0 != s1) *shared = true;
             for (int r = w[i].row; r < w[i].row + w[i].rows; r++) {
@@ -106,6 +124,7 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
         total += (size_t)tok[r / G].parts;
     }
     CHECK(parts.size() == total);
+    for (int r = 0; r < T * G; r++) CHECK(tok[r / G].parts == 1 || joined.count(r) || apart.count(r / G));
 }
 
 int main(int argc, char **argv)
