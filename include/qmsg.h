@@ -330,6 +330,24 @@ int qmsg_attn_append_device(qmsg_ctx *ctx, int id, int layer, float *d_qr, const
  * Enqueued without waiting. */
 int qmsg_attn_device(qmsg_ctx *ctx, int id, int layer, const float *d_q, float *d_out);
 
+/* The attention half of qms_forward's layer loop (src/model.c:1277-1282) for the batch's T new tokens, on device
+ * rows d_h [T][n_embd] updated in place: xn = rmsnorm(h, attn_norm), q/k/v = their products with xn,
+ * qmsg_attn_append_device, qmsg_attn_device, h += output product. qmsg_moe_chain is the other half.
+ * qmsg_attn_mats names the layer's q, k, v and output matrices (ids of qmsg_mat_upload or
+ * qmsg_gguf_upload_mat, shapes checked) and its attn_norm (n_embd host floats, NULL: unit weights).
+ * A captured call's products take the T of the batch that is set when it is captured: replay it
+ * on batches of as many new tokens. Enqueued without waiting. */
+int qmsg_attn_mats(qmsg_ctx *ctx, int id, int layer, const int *ids, const float *attn_norm);
+int qmsg_attn_layer(qmsg_ctx *ctx, int id, int layer, float *d_h, float eps);
+
+/* The attention keys of read_cfg (src/model.c:278-310) of a qwen3moe file: n_head, n_head_kv, head_dim, n_layer,
+ * rope_base and qk_norm = 1; the other fields stay as they are. */
+int qmsg_gguf_attn_cfg(const qmsg_gguf *g, qmsg_attn_cfg *cfg);
+/* The attention lines of qms_model_load for file layers first .. first+n-1 into the layers of the same index:
+ * blk.L.attn_{q,k,v,output}.weight, attn_norm, attn_q_norm and attn_k_norm (F32; without qk_norm the last
+ * two are not read). Shapes are checked before any memory changes. */
+int qmsg_gguf_attn_upload(qmsg_ctx *ctx, const qmsg_gguf *g, int id, int first, int n);
+
 /* ------------------------------------------------------------------ device buffers ---- */
 
 /* No reference counterpart: device memory owned by the context (freed by qmsg_destroy). */

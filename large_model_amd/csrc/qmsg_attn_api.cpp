@@ -2,9 +2,11 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdio>
 #include <cstring>
 
 #include "qmsg_ctx.h"
+#include "qmsg_gguf.h"
 
 using namespace qmsg;
 
@@ -309,6 +311,148 @@ int qmsg_attn_device(qmsg_ctx *c, int id, int layer, const float *d_q, float *d_
     k.q = d_q;
     k.out = d_out;
     LAUNCH(c, "attend", launch_attend(k, a->cfg.type, a->cfg.head_dim, live_grid(c), c->stream));
+    return QMSG_OK;
+}
+
+/* The dense matrices of a layer's q, k, v and output products, checked against the attention's heads. */
+static int check_mats(qmsg_ctx *c, const AttnStore &a, const int *ids, const char *what)
+{
+    const int64_t E = c->cfg.n_embd, Q = (int64_t)a.cfg.n_head * a.cfg.head_dim, KV = (int64_t)a.cfg.n_head_kv * a.cfg.head_dim;
+    const struct { int64_t rows, cols; const char *name; } want[4] = { { Q, E, "q" }, { KV, E, "k" }, { KV, E, "v" }, { E, Q, "output" } };
+    for (int i = 0; i < 4; i++) {
+        if (ids[i] < 0 || ids[i] >= (int)c->mats.size()) return fail(c, QMSG_E_INVALID, "%s: matrix id %d unknown", what, ids[i]);
+        const DenseStore &m = c->mats[(size_t)ids[i]];
+        if (m.rows != want[i].rows || m.cols != want[i].cols)
+            return fail(c, QMSG_E_INVALID, "%s: %s matrix is %lld x %lld, expected %lld x %lld", what, want[i].name, (long long)m.rows,
+                        (long long)m.cols, (long long)want[i].rows, (long long)want[i].cols);
+    }
+    return QMSG_OK;
+}
+
+int qmsg_attn_mats(qmsg_ctx *c, int id, int layer, const int *ids, const float *attn_norm)
+{
+    if (!c || !ids) return QMSG_E_INVALID;
+    int rc = QMSG_OK;
+    AttnStore *a = find_attn(c, id, layer, "qmsg_attn_mats", &rc);
+    if (!a) return rc;
+    if ((rc = check_mats(c, *a, ids, "qmsg_attn_mats"))) return rc;
+    if (rmsnorm_lds_bytes(c->cfg.n_embd) > 160 * 1024)
+        return fail(c, QMSG_E_UNSUPPORTED, "qmsg_attn_mats: rows of %d floats exceed the norm's LDS", c->cfg.n_embd);
+    HIP_TRY(c, hipSetDevice(c->device));
+    HIP_TRY(c, hipStreamSynchronize(c->stream));
+    AttnLayer &l = a->layers[(size_t)layer];
+    NO_THROW(c, "qmsg_attn_mats", {
+        if (!a->rows) {
+            const size_t T = (size_t)a->cfg.max_tokens, Q = (size_t)a->cfg.n_head * (size_t)a->cfg.head_dim, KV = (size_t)a->cfg.n_head_kv * (size_t)a->cfg.head_dim;
+            if ((rc = dev_alloc(c, (void **)&a->rows, T * (2 * (size_t)c->cfg.n_embd + 2 * Q + 2 * KV) * 4, a->allocs))) return rc;
+        }
+        if ((rc = set_vector(c, &l.norm, attn_norm, (size_t)c->cfg.n_embd))) return rc;
+    })
+    memcpy(l.mats, ids, sizeof l.mats);
+    return QMSG_OK;
+}
+
+int qmsg_attn_layer(qmsg_ctx *c, int id, int layer, float *d_h, float eps)
+{
+    if (!c) return QMSG_E_INVALID;
+    int rc = QMSG_OK;
+    AttnStore *a = find_attn(c, id, layer, "qmsg_attn_layer", &rc);
+    if (!a) return rc;
+    const AttnLayer &l = a->layers[(size_t)layer];
+    if (l.mats[0] < 0) return fail(c, QMSG_E_INVALID, "qmsg_attn_layer: layer %d has no matrices", layer);
+    if (!d_h || ((uintptr_t)d_h & 15)) return fail(c, QMSG_E_INVALID, "qmsg_attn_layer: d_h must be 16-byte aligned");
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(c, QMSG_E_INVALID, "qmsg_attn_layer: eps %g", (double)eps);
+    const int T = a->plan.h.n_tok, E = c->cfg.n_embd;
+    if (T == 0) return QMSG_OK;
+    HIP_TRY(c, hipSetDevice(c->device));
+    const size_t t = (size_t)T, Q = (size_t)a->cfg.n_head * (size_t)a->cfg.head_dim, KV = (size_t)a->cfg.n_head_kv * (size_t)a->cfg.head_dim;
+    float *x = a->rows, *q = x + t * (size_t)E, *k = q + t * Q, *v = k + t * KV, *out = v + t * KV, *o = out + t * Q;
+    LAUNCH(c, "rmsnorm", launch_rmsnorm(d_h, nullptr, l.norm, x, T, E, eps, c->norm_walk, c->d_walked, c->stream));
+    float *const ys[3] = { q, k, v };
+    float *const yo[1] = { o };
+    NO_THROW(c, "qmsg_attn_layer", {
+        if ((rc = qmsg_matmul_n_device(c, l.mats, 3, x, T, ys))) return rc;
+        if ((rc = qmsg_attn_append_device(c, id, layer, q, q, k, v, eps))) return rc;
+        if ((rc = qmsg_attn_device(c, id, layer, q, out))) return rc;
+        if ((rc = qmsg_matmul_n_device(c, l.mats + 3, 1, out, T, yo))) return rc;
+    })
+    LAUNCH(c, "add", launch_add_rows(d_h, o, t * (size_t)E, c->stream));
+    return QMSG_OK;
+}
+
+int qmsg_gguf_attn_cfg(const qmsg_gguf *g, qmsg_attn_cfg *f)
+{
+    if (!g || !f) return QMSG_E_INVALID;
+    qmsg_cfg moe;
+    int n_layer = 0;
+    int rc = qmsg_gguf_moe_cfg(g, &moe, &n_layer, nullptr);
+    if (rc) return rc;
+    int64_t v[2];
+    const char *names[2] = { "qwen3moe.attention.head_count", "qwen3moe.attention.head_count_kv" };
+    for (int i = 0; i < 2; i++) {
+        if ((rc = qmsg_gguf_get_int(g, names[i], &v[i]))) return rc;
+        if (v[i] <= 0 || v[i] > 1 << 20) return fail(nullptr, QMSG_E_INVALID, "qmsg_gguf_attn_cfg: %s = %lld", names[i], (long long)v[i]);
+    }
+    int64_t dk = moe.n_embd / v[0], dv;
+    if (g->scalar("qwen3moe.attention.key_length") && (rc = qmsg_gguf_get_int(g, "qwen3moe.attention.key_length", &dk))) return rc;
+    dv = dk;
+    if (g->scalar("qwen3moe.attention.value_length") && (rc = qmsg_gguf_get_int(g, "qwen3moe.attention.value_length", &dv))) return rc;
+    if (dk != dv || dk <= 0 || dk > 1 << 20)
+        return fail(nullptr, QMSG_E_UNSUPPORTED, "qmsg_gguf_attn_cfg: key_length %lld, value_length %lld", (long long)dk, (long long)dv);
+    double base = 10000.0;
+    if (g->scalar("qwen3moe.rope.freq_base") && (rc = qmsg_gguf_get_float(g, "qwen3moe.rope.freq_base", &base))) return rc;
+    f->n_head = (int)v[0];
+    f->n_head_kv = (int)v[1];
+    f->head_dim = (int)dk;
+    f->n_layer = n_layer;
+    f->qk_norm = 1;
+    f->rope_base = (float)base;
+    return QMSG_OK;
+}
+
+int qmsg_gguf_attn_upload(qmsg_ctx *c, const qmsg_gguf *g, int id, int first, int n)
+{
+    if (!c || !g || n < 0) return QMSG_E_INVALID;
+    int rc = QMSG_OK;
+    AttnStore *a = find_attn(c, id, 0, "qmsg_gguf_attn_upload", &rc);
+    if (!a) return rc;
+    if (first < 0 || first > a->cfg.n_layer - n)
+        return fail(c, QMSG_E_RANGE, "layers %d .. %d outside [0, %d)", first, first + n - 1, a->cfg.n_layer);
+    const int64_t E = c->cfg.n_embd, D = a->cfg.head_dim, Q = a->cfg.n_head * D, KV = a->cfg.n_head_kv * D;
+    const struct { const char *name; int64_t ne0, ne1; } want[7] = {
+        { "attn_q", E, Q }, { "attn_k", E, KV }, { "attn_v", E, KV }, { "attn_output", Q, E }, { "attn_norm", E, 1 }, { "attn_q_norm", D, 1 }, { "attn_k_norm", D, 1 } };
+    const int n_vec = a->cfg.qk_norm ? 3 : 1;
+    NO_THROW(c, "qmsg_gguf_attn_upload", {
+        /* every layer's tensors are checked before any device memory changes */
+        std::vector<const qmsg_tensor *> t((size_t)n * 7, nullptr);
+        for (int l = 0; l < n; l++)
+            for (int k = 0; k < 4 + n_vec; k++) {
+                char name[96];
+                snprintf(name, sizeof name, "blk.%d.%s.weight", first + l, want[k].name);
+                const int i = gguf_find(g, name);
+                if (i < 0) return fail(c, QMSG_E_INVALID, "model: missing tensor %s", name);
+                const qmsg_tensor &x = g->tensors[(size_t)i];
+                if (x.ne[0] != want[k].ne0 || x.ne[1] != want[k].ne1 || x.ne[2] != 1 || x.ne[3] != 1)
+                    return fail(c, QMSG_E_INVALID, "model: %s expected [%lld x %lld], got ne=[%lld,%lld,%lld]", name, (long long)want[k].ne0,
+                                (long long)want[k].ne1, (long long)x.ne[0], (long long)x.ne[1], (long long)x.ne[2]);
+                if (k >= 4 && x.type != QMSG_T_F32) return fail(c, QMSG_E_UNSUPPORTED, "%s: norms are F32 (got type %d)", name, x.type);
+                t[(size_t)l * 7 + (size_t)k] = &x;
+            }
+        std::vector<float> vec[3];
+        for (int l = 0; l < n; l++) {
+            int ids[4];
+            for (int k = 0; k < 4; k++)
+                if ((rc = qmsg_gguf_upload_mat(c, g, t[(size_t)l * 7 + (size_t)k]->name, &ids[k]))) return rc;
+            for (int k = 0; k < n_vec; k++) {
+                const qmsg_tensor &x = *t[(size_t)l * 7 + 4 + (size_t)k];
+                vec[k].resize((size_t)x.ne[0]);
+                if (gguf_pread(g, x.shard, x.off, (uint64_t)x.ne[0] * 4, vec[k].data()))
+                    return fail(c, QMSG_E_INVALID, "gguf upload: read failed for %s", x.name);
+            }
+            if ((rc = qmsg_attn_mats(c, id, first + l, ids, vec[0].data()))) return rc;
+            if (n_vec == 3 && (rc = qmsg_attn_norms(c, id, first + l, vec[1].data(), vec[2].data()))) return rc;
+        }
+    })
     return QMSG_OK;
 }
 

@@ -136,6 +136,10 @@ _SIGS = {
     "qmsg_attn_batch": (_I, [_P, _I, _I, _P, _P, _P, _I]),
     "qmsg_attn_append_device": (_I, [_P, _I, _I, _P, _P, _P, _P, ctypes.c_float]),
     "qmsg_attn_device": (_I, [_P, _I, _I, _P, _P]),
+    "qmsg_attn_mats": (_I, [_P, _I, _I, _P, _P]),
+    "qmsg_attn_layer": (_I, [_P, _I, _I, _P, ctypes.c_float]),
+    "qmsg_gguf_attn_cfg": (_I, [_P, ctypes.POINTER(_AttnCfg)]),
+    "qmsg_gguf_attn_upload": (_I, [_P, _P, _I, _I, _I]),
     "qmsg_device_info": (_I, [_P, ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(ctypes.c_uint64),
                               ctypes.c_char_p, _I]),
 }
@@ -241,6 +245,14 @@ class Gguf:
             self._raise(st)
         return {"n_embd": cfg.n_embd, "n_expert": cfg.n_expert, "n_used": cfg.n_used, "n_ff_exp": cfg.n_ff_exp,
                 "n_layer": nl.value, "eps": eps.value}
+
+    def attn_cfg(self) -> dict:
+        """read_cfg's attention keys (src/model.c:278-310): n_head, n_head_kv, head_dim, n_layer, rope_base."""
+        cfg = _AttnCfg()
+        st = lib.qmsg_gguf_attn_cfg(self._h, ctypes.byref(cfg))
+        if st != 0:
+            self._raise(st)
+        return {k: getattr(cfg, k) for k in ("n_head", "n_head_kv", "head_dim", "n_layer", "rope_base")}
 
 
 class Context:
@@ -469,6 +481,27 @@ class Context:
     def attn_device(self, attn: int, layer: int, d_q: int, d_out: int):
         """d_out = the batch's attention over the cache, each token seeing its sequence up to its own position."""
         self._check(lib.qmsg_attn_device(self._h, attn, layer, d_q, d_out))
+
+    def attn_mats(self, attn: int, layer: int, ids, attn_norm: Optional[np.ndarray] = None):
+        """A layer's q, k, v and output matrices (ids) and its attn_norm (None: unit weights)."""
+        if len(ids) != 4:
+            raise ValueError("ids are those of q, k, v and output")
+        w = None if attn_norm is None else np.ascontiguousarray(attn_norm, np.float32)
+        if w is not None and w.size != self.E:
+            raise ValueError(f"attn_norm has {self.E} weights")
+        self._check(lib.qmsg_attn_mats(self._h, attn, layer, (_I * 4)(*ids), _ptr(w)))
+
+    def attn_layer(self, attn: int, layer: int, d_h: int, eps: float = 1e-6):
+        """h += output(attention(q, k, v of rmsnorm(h))) for the batch's rows d_h (qms_forward, src/model.c:1277-1282)."""
+        self._check(lib.qmsg_attn_layer(self._h, attn, layer, d_h, eps))
+
+    def attn_from_gguf(self, g: Gguf, **sizes) -> int:
+        """An attention with the file's heads and rotation and every layer's matrices and norms; sizes: type_, page,
+        n_page, max_seq, max_tokens, max_pages, d_k and d_v of attn_create."""
+        c = g.attn_cfg()
+        i = self.attn_create(c["n_head"], c["n_head_kv"], c["head_dim"], n_layer=c["n_layer"], rope_base=c["rope_base"], **sizes)
+        self._check(lib.qmsg_gguf_attn_upload(self._h, g._h, i, 0, c["n_layer"]))
+        return i
 
     # ---------------------------------------------------------------- device buffers / timing
     def device_alloc(self, nbytes: int) -> int:

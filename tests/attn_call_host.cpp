@@ -22,6 +22,14 @@ hipError_t last = hipSuccess;
 bool capturing = false;
 std::vector<qmsg::AttnCall> attends;
 std::vector<qmsg::AttnAppend> appends;
+struct Step {
+    const char *name;
+    const float *in;
+    float *out;
+    int n;
+    const float *w;
+};
+std::vector<Step> steps;
 
 hipError_t ret(hipError_t e)
 {
@@ -75,6 +83,21 @@ hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, hipMemcpyKind, hipSt
 namespace qmsg {
 thread_local const LaunchTimer *g_launch_timer = nullptr;
 hipError_t launch_attend(const AttnCall &a, int, int, int, hipStream_t) { attends.push_back(a); return hipGetLastError(); }
+hipError_t launch_rmsnorm(float *x, const float *, const float *w, float *y, int T, int E, float, int, unsigned long long *, hipStream_t)
+{
+    steps.push_back({ "rmsnorm", x, y, T * E, w });
+    return hipGetLastError();
+}
+hipError_t launch_add_rows(float *h, const float *d, size_t n, hipStream_t)
+{
+    steps.push_back({ "add", d, h, (int)n, nullptr });
+    return hipGetLastError();
+}
+hipError_t launch_dense(const DenseArgs &a, int, uint8_t *, uint64_t, bool *, hipStream_t)
+{
+    for (int i = 0; i < a.nm; i++) steps.push_back({ "dense", a.x, a.m[i].y, a.T * a.m[i].rows, nullptr });
+    return hipGetLastError();
+}
 hipError_t launch_attn_append(const AttnAppend &b, int, int, int, hipStream_t) { appends.push_back(b); return hipGetLastError(); }
 }  // namespace qmsg
 
@@ -278,6 +301,50 @@ static void calls()
     CHECK(qmsg_attn_cache(ctx, plain, &k, &v) == QMSG_OK && k == kK && v == kV);
 }
 
+static int mat(int64_t rows, int64_t cols)
+{
+    static uint8_t data[16];
+    const qmsg_mat m = { QMSG_T_Q4_0, rows, cols, (uint64_t)cols / 32 * 18, data };
+    int id = -1;
+    CHECK(qmsg_mat_upload(ctx, &m, &id) == QMSG_OK);
+    return id;
+}
+
+static void layers()
+{
+    const int id = make();
+    const int q[1] = { 3 }, kv[1] = { 20 };
+    const int32_t pages[2] = { 1, 2 };
+    const int good[4] = { mat(512, 256), mat(128, 256), mat(128, 256), mat(256, 512) };
+    float norm[256] = { 1 };
+    float *const h = (float *)(8ull << 20);
+    CHECK(qmsg_attn_batch(ctx, id, 1, q, kv, pages, 2) == QMSG_OK);
+    CHECK(qmsg_attn_layer(ctx, id, 0, h, 1e-6f) == QMSG_E_INVALID);           /* no matrices yet */
+    for (int k = 0; k < 4; k++)
+        for (int bad : { -1, 99, good[(k + 1) % 4 == 2 ? 3 : (k + 1) % 4] }) {
+            int ids[4] = { good[0], good[1], good[2], good[3] };
+            ids[k] = bad;
+            CHECK(qmsg_attn_mats(ctx, id, 0, ids, norm) == QMSG_E_INVALID);
+        }
+    CHECK(qmsg_attn_mats(ctx, id, 2, good, norm) == QMSG_E_RANGE && qmsg_attn_mats(ctx, id + 1, 0, good, norm) == QMSG_E_INVALID);
+    CHECK(qmsg_attn_mats(ctx, id, 0, nullptr, norm) == QMSG_E_INVALID && qmsg_attn_mats(nullptr, id, 0, good, norm) == QMSG_E_INVALID);
+    CHECK(qmsg_attn_mats(ctx, id, 1, good, norm) == QMSG_OK && qmsg_attn_mats(ctx, id, 0, good, nullptr) == QMSG_OK);
+    CHECK(qmsg_attn_layer(ctx, id, 2, h, 1e-6f) == QMSG_E_RANGE && qmsg_attn_layer(ctx, id + 1, 0, h, 1e-6f) == QMSG_E_INVALID);
+    CHECK(qmsg_attn_layer(ctx, id, 1, nullptr, 1e-6f) == QMSG_E_INVALID && qmsg_attn_layer(ctx, id, 1, h + 1, 1e-6f) == QMSG_E_INVALID);
+    CHECK(qmsg_attn_layer(ctx, id, 1, h, NAN) == QMSG_E_INVALID && qmsg_attn_layer(nullptr, id, 1, h, 1e-6f) == QMSG_E_INVALID && steps.empty());
+    CHECK(qmsg_attn_layer(ctx, id, 1, h, 1e-6f) == QMSG_OK);
+    /* norm, q, k, v, append, attention, output, residual: each on what the one before left */
+    CHECK(steps.size() == 6 && appends.size() == 1 && attends.size() == 1);
+    const float *x = steps[0].out;
+    CHECK(steps[0].in == h && steps[0].n == 3 * 256 && steps[0].w && steps[1].in == x && steps[2].in == x && steps[3].in == x);
+    CHECK(steps[1].n == 3 * 512 && steps[2].n == 3 * 128 && steps[1].out + steps[1].n <= steps[2].out && steps[2].out + steps[2].n <= steps[3].out);
+    CHECK(appends[0].q == steps[1].out && appends[0].qr == steps[1].out && appends[0].k == steps[2].out && appends[0].v == steps[3].out);
+    CHECK(attends[0].q == steps[1].out && steps[4].in == attends[0].out && steps[5].in == steps[4].out && steps[5].out == h && steps[5].n == 3 * 256);
+    CHECK(attends[0].out >= steps[3].out + steps[3].n && steps[4].out == attends[0].out + 3 * 512);
+    CHECK(appends[0].c.k == ctx->attns[(size_t)id]->k + ctx->attns[(size_t)id]->layer_bytes);
+    CHECK(qmsg_attn_batch(ctx, id, 0, nullptr, nullptr, nullptr, 0) == QMSG_OK && qmsg_attn_layer(ctx, id, 1, h, 1e-6f) == QMSG_OK && steps.size() == 6);
+}
+
 int main(int argc, char **argv)
 {
     const std::string s = argc > 1 ? argv[1] : "";
@@ -287,6 +354,7 @@ int main(int argc, char **argv)
     else if (s == "memory") memory();
     else if (s == "batches") batches();
     else if (s == "calls") calls();
+    else if (s == "layers") layers();
     else return 2;
     qmsg_destroy(ctx);
     ctx = nullptr;
