@@ -211,13 +211,15 @@ int qmsg_attn_cache(qmsg_ctx *c, int id, void **d_k, void **d_v)
     return QMSG_OK;
 }
 
-/* n host floats to a device vector made on first use; NULL frees it (unit weights). */
+/* n host floats to a device vector made on first use. NULL: ones, where there is one (a captured call may hold
+ * it, so it stays). */
 static int set_vector(qmsg_ctx *c, float **d, const float *w, size_t n)
 {
+    if (!w && !*d) return QMSG_OK;
+    std::vector<float> ones;
     if (!w) {
-        hipFree(*d);
-        *d = nullptr;
-        return QMSG_OK;
+        ones.assign(n, 1.0f);
+        w = ones.data();
     }
     if (!*d) {
         std::vector<void *> tmp;
@@ -259,6 +261,7 @@ int qmsg_attn_batch(qmsg_ctx *c, int id, int n_seq, const int *q_len, const int 
         const std::string err = attn_plan(a->shape, c->n_cu, n_seq, q_len, kv_len, pages, stride, &a->plan);
         if (!err.empty()) return fail(c, QMSG_E_INVALID, "qmsg_attn_batch: %s", err.c_str());
         rc = send_plan(c, *a, a->plan);
+        if (rc) a->plan.h = AttnHdr{};              /* no batch, rather than another than the device's */
     })
     return rc;
 }

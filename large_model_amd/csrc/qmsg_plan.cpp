@@ -41,25 +41,14 @@ struct Tile {
 
 int kind_of(int rows) { return rows <= attn_rows(kAttnFew, 1) ? kAttnFew : kAttnMany; }
 
-/* Blocks that a CU holds, the fewest keys worth a block, and what an item costs besides its keys, in keys. */
+/* Blocks that a CU holds, the fewest keys worth a block, and what an item costs besides its keys, in keys. us by
+ * fewest keys: one token over 513 keys 3.9 at 256, 4.1 in one piece of 513 (alone 22 / 24); 8 sequences of 5
+ * drafted tokens 16.7 at 256, 15.7 at 384, 15.0 at 512, 15.7 at 768 (attention alone 23.8, 21.2, 22.7, 28.9); three fp32 prompts
+ * to 701 tokens 26.2 at 64 and 128, 27.2 at 256. By an item's cost of 64 / 128 / 192 / 256 keys: 64 sequences on
+ * 8192 shared keys 44.4 / 42.7 / 43.0 / 41.7, the fp32 prompts 17.9 / 18.2 / 17.3 / 17.5. */
 constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };
-#ifndef FEWK
-#define FEWK 256
-#endif
-#ifndef MANYK
-#define MANYK 384
-#endif
-#ifndef MANYK32
-#define MANYK32 128
-#endif
-#ifndef C0F
-#define C0F 128
-#endif
-#ifndef C0M
-#define C0M 64
-#endif
-constexpr int kMinKeys[kAttnKinds] = { FEWK, MANYK }, kMinKeysF32 = MANYK32;
-constexpr int kItemCost[kAttnKinds] = { C0F, C0M };
+constexpr int kMinKeys[kAttnKinds] = { 256, 384 }, kMinKeysF32 = 128;
+constexpr int kItemCost[kAttnKinds] = { 128, 192 };
 /* Cuts fall on multiples of this many keys from a tile's first. */
 constexpr int kCut = 64;
 
@@ -164,15 +153,14 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
                 b++;
             }
             const bool group = b - a > 1;
-            if (group) {
-                if (keys > kv_len[i] - q_len[i]) keys = kv_len[i] - q_len[i];
-                keys = keys / P * P;
-                seg.push_back({ first[(size_t)i], n_tok, 0, keys, table[(size_t)i], -1, kind_of(n_tok * G), 0 });
-            }
+            if (group) seg.push_back({ first[(size_t)i], n_tok, 0, keys, table[(size_t)i], -1, kind_of(n_tok * G), 0 });
             for (size_t c = a; c < b; c++) {
-                const int j = used[c];
+                /* a group's own keys in the launch of its shared ones (64 sequences on 8192 shared keys: 44.5 us,
+                 * in a launch of their own 51.3), which reads keys for few rows as fast (allotting all
+                 * decoding to it: 32 sequences 53.5 us against 54.7) but has more parts to join */
+                const int j = used[c], kind = kind_of((group ? n_tok : q_len[j]) * G);
                 seg.push_back({ first[(size_t)j], q_len[j], group ? keys : 0, kv_len[j], table[(size_t)j],
-                                kv_len[j] - q_len[j], kind_of(q_len[j] * G), 0 });
+                                kv_len[j] - q_len[j], kind, 0 });
             }
             a = b;
         }
@@ -281,7 +269,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     for (int share = 1; share >= 0 && !fits; share--) {
         segments(share != 0);
         make_tiles();
-        for (int64_t coarser = 1; coarser <= (int64_t)1 << 32 && !fits; coarser *= 2) {
+        for (int64_t coarser = 1; coarser <= (int64_t)1 << 24 && !fits; coarser *= 2) {
             for (int k = 0; k < kAttnKinds; k++) cut_tiles(k, coarser);
             fits = count_parts();
         }

@@ -19,7 +19,7 @@ namespace {
 std::set<void *> live;                 /* device and pinned memory, events */
 int fail_at = -1, allocs = 0, set_devices = 0;
 hipError_t last = hipSuccess;
-bool capturing = false;
+bool capturing = false, copy_fails = false;
 std::vector<qmsg::AttnCall> attends;
 std::vector<qmsg::AttnAppend> appends;
 struct Step {
@@ -77,7 +77,12 @@ hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus *s)
 }
 hipError_t hipMemset(void *, int, size_t) { return hipSuccess; }
 hipError_t hipMemcpy(void *, const void *, size_t, hipMemcpyKind) { return hipSuccess; }
-hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, hipMemcpyKind, hipStream_t) { memcpy(d, s, n); return hipSuccess; }
+hipError_t hipMemcpyAsync(void *d, const void *s, size_t n, hipMemcpyKind, hipStream_t)
+{
+    if (copy_fails) return ret(hipErrorInvalidValue);
+    memcpy(d, s, n);
+    return hipSuccess;
+}
 }
 
 namespace qmsg {
@@ -234,6 +239,12 @@ static void batches()
     expect(QMSG_E_INVALID, 3, q, kv, &pages[0][0], 8);
     capturing = false;
     CHECK(qmsg_attn_batch(ctx, id + 1, 0, q, kv, &pages[0][0], 8) == QMSG_E_INVALID && qmsg_attn_batch(nullptr, id, 0, q, kv, &pages[0][0], 8) == QMSG_E_INVALID);
+    /* a batch that does not reach the device leaves none */
+    copy_fails = true;
+    CHECK(qmsg_attn_batch(ctx, id, 3, q, kv, &pages[0][0], 8) == QMSG_E_DEVICE && h->n_tok == 0 && last == hipSuccess);
+    copy_fails = false;
+    CHECK(qmsg_attn_device(ctx, id, 0, kQ, kQr) == QMSG_OK && attends.empty());
+    CHECK(qmsg_attn_batch(ctx, id, 3, q, kv, &pages[0][0], 8) == QMSG_OK && h->n_tok == 3);
     CHECK(qmsg_attn_batch(ctx, id, 0, nullptr, nullptr, nullptr, 0) == QMSG_OK && h->n_tok == 0);
 }
 
@@ -293,6 +304,8 @@ static void calls()
     void *k = nullptr, *v = nullptr;
     CHECK(qmsg_attn_norms(ctx, id, 2, w, w) == QMSG_E_RANGE && qmsg_attn_norms(ctx, id + 1, 0, w, w) == QMSG_E_INVALID);
     CHECK(qmsg_attn_norms(ctx, id, 1, w, nullptr) == QMSG_OK && qmsg_attn_norms(ctx, id, 1, nullptr, w) == QMSG_OK);
+    /* the vector stays where a captured call may read it */
+    CHECK(ctx->attns[(size_t)id]->layers[1].qw && live.count(ctx->attns[(size_t)id]->layers[1].qw));
     CHECK(qmsg_attn_cache(ctx, id, &k, nullptr) == QMSG_E_INVALID && qmsg_attn_cache(ctx, -1, &k, &v) == QMSG_E_INVALID && qmsg_attn_cache(ctx, id, &k, &v) == QMSG_OK && k && v);
     qmsg_attn_cfg f = config();
     f.qk_norm = 0;
