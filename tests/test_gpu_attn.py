@@ -55,6 +55,7 @@ LENS = {
     "ragged": [(1, 300), (0, 40), (1, 1), (1, 777), (0, 0), (1, 129)],
     "draft": [(5, 5), (3, 260), (8, 515)],
     "prompt": [(33, 33), (130, 130), (1, 90), (65, 301)],
+    "chunk": [(20, 2000), (1, 1200), (37, 1500)],
 }
 
 
@@ -63,7 +64,7 @@ LENS = {
 @pytest.mark.parametrize("lens", list(LENS))
 def test_attention(ctx, lens, heads, type_):
     H, kv, D = heads
-    page = {"one": 16, "ends": 16, "ragged": 64, "draft": 32, "prompt": 128}[lens]
+    page = {"one": 16, "ends": 16, "ragged": 64, "draft": 32, "prompt": 128, "chunk": 64}[lens]
     print(f"[case] {lens} {heads} type {type_}", flush=True)
     b = Batch(LENS[lens], page, seed=H + D)
     k, v = values(b, kv, D, type_, 1)
@@ -108,7 +109,7 @@ def test_shared_prefix(ctx, what, type_):
 
 @pytest.mark.parametrize("type_", [F16, F32])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("n", [6, 150])
+@pytest.mark.parametrize("n", [3, 6, 150])
 def test_what_a_row_does_not_see(ctx, type_, bad, n):
     """Infinities and NaN in later tokens' keys and values do not reach earlier rows; those that see them get them."""
     H, kv, D = 8, 2, 64
@@ -141,6 +142,21 @@ def test_score_and_query_ranges(ctx, type_):
     q[3, 4] *= 500
     q[4] *= np.float32(2.0) ** np.arange(-20, 12, 2)[:, None].astype(np.float32)
     print(f"[case] ranges, type {type_}", flush=True)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    check(got, *attend64(b, q, k, v, D ** -0.5))
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("what", ["long", "long_group", "many", "more_tiles_than_blocks"])
+def test_batch_sizes(ctx, what, type_):
+    """Parts for the join kernel, more sequences than blocks, more tiles than the card holds blocks."""
+    H, kv, D = 8, 1, 64
+    lens, shared = {"long": ([(1, 20011)], 0), "long_group": ([(1, 9100), (1, 9500)], 9088), "many": ([(1, 1 + 7 * i % 61) for i in range(300)], 0),
+                    "more_tiles_than_blocks": ([(150, 150 + i % 5) for i in range(110)], 0)}[what]
+    print(f"[case] {what}, type {type_}", flush=True)
+    b = Batch(lens, 64, shared, seed=24)
+    k, v = values(b, kv, D, type_, 25, shared)
+    q = (2 * np.random.default_rng(26).standard_normal((b.T, H, D))).astype(np.float32)
     got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
     check(got, *attend64(b, q, k, v, D ** -0.5))
 
