@@ -75,7 +75,7 @@ size_t attn_blob_bytes(const AttnShape &s)
 }
 
 std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len, const int *kv_len, const int32_t *pages,
-                      int stride, AttnPlan *p)
+                      int stride, AttnPlan *p, int64_t min_saved)
 {
     const int G = s.heads / s.kv_heads, P = s.page;
     if (n_seq < 0 || n_seq > s.max_seq) return text("%d sequences outside [0, max_seq=%d]", n_seq, s.max_seq);
@@ -138,7 +138,8 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     for (int i = 0; i < n_seq; i++)
         if (q_len[i]) used.push_back(i);
     std::vector<Segment> seg;
-    auto segments = [&](bool share) {
+    auto segments = [&](bool share) -> int64_t {               /* bytes of keys and values that sharing saves */
+        int64_t saved = 0;
         seg.clear();
         for (size_t a = 0; a < used.size();) {
             const int i = used[a];
@@ -153,6 +154,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
                 b++;
             }
             const bool group = b - a > 1;
+            if (group) saved += (int64_t)keys * (int64_t)(b - a - 1) * 2 * s.D * (s.type == 1 ? 2 : 4) * s.kv_heads;
             if (group) seg.push_back({ first[(size_t)i], n_tok, 0, keys, table[(size_t)i], -1, kind_of(n_tok * G), 0 });
             for (size_t c = a; c < b; c++) {
                 /* a group's own keys in the launch of its shared ones (64 sequences on 8192 shared keys: 44.5 us,
@@ -164,6 +166,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
             }
             a = b;
         }
+        return saved;
     };
     const size_t part_rows = attn_part_rows(s);
     std::vector<Tile> tiles;
@@ -267,7 +270,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     };
     bool fits = false;
     for (int share = 1; share >= 0 && !fits; share--) {
-        segments(share != 0);
+        if (segments(share != 0) < min_saved && share) continue;
         make_tiles();
         for (int64_t coarser = 1; coarser <= (int64_t)1 << 24 && !fits; coarser *= 2) {
             for (int k = 0; k < kAttnKinds; k++) cut_tiles(k, coarser);

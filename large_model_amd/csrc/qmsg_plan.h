@@ -82,10 +82,15 @@ struct AttnPlan {
     int64_t batches = 0;
 };
 
+/* Sharing that saves fewer bytes than this is left: its parts need a launch of their own to be joined. us (alone,
+ * host round trip included) by the MB saved, shared / not: 4.3 6.6 / 3.7 (25.7 / 20.1), 16.5 8.9 / 11.2 (32.3 / 26.3),
+ * 25.2 8.0 / 9.3 (30.4 / 27.2), 32.4 7.4 / 10.5 (27.4 / 27.1). */
+constexpr int64_t kMinSaved = 24 << 20;
+
 /* Plan n_seq sequences: q_len[i] new tokens, the last of kv_len[i] tokens, on pages
  * [i * stride ..]. Returns an empty string, or what is wrong with the batch (p keeps its last). */
 std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len, const int *kv_len, const int32_t *pages,
-                      int stride, AttnPlan *p);
+                      int stride, AttnPlan *p, int64_t min_saved = kMinSaved);
 
 }  // namespace qmsg
 

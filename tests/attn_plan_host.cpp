@@ -160,7 +160,8 @@ int main(int argc, char **argv)
             for (int j = 0; j < (kv[i] + s.page - 1) / s.page; j++)
                 pages[(size_t)i * stride + j] = j < shared && !(batch % 2 && i > n_seq / 2 && j > shared / 2) ? deal[(size_t)j] : deal[(size_t)at++];
         AttnPlan p;
-        const std::string err = attn_plan(s, pick(0, 1) ? 256 : 4, n_seq, q.data(), kv.data(), pages.data(), stride, &p);
+        const int64_t min_saved = batch % 4 ? 0 : kMinSaved;       /* small batches share too, or few do */
+        const std::string err = attn_plan(s, pick(0, 1) ? 256 : 4, n_seq, q.data(), kv.data(), pages.data(), stride, &p, min_saved);
         if (!err.empty()) fprintf(stderr, "%s\n", err.c_str());
         CHECK(err.empty());
         bool sh = false;

@@ -91,19 +91,23 @@ def test_every_key_counts_once(ctx, page, type_):
 @pytest.mark.parametrize("type_", [F16, F32])
 @pytest.mark.parametrize("what", ["one", "two_runs", "tokens", "wide", "idle"])
 def test_shared_prefix(ctx, what, type_):
-    H, kv, D, page = 32, 4, 128, 32
+    H, kv, D, page = (64, 4, 128, 32) if what == "wide" else (32, 16, 128, 32)     # enough bytes to be worth sharing
     shared, runs, lens = {
-        "one": (512, None, [(1, 513), (1, 700), (1, 900), (1, 530)]),
-        "two_runs": (320, [3, 1, 2], [(1, 321), (1, 480), (1, 322), (1, 333), (1, 600), (1, 345)]),
-        "tokens": (288, None, [(3, 300), (1, 289), (2, 290), (6, 400)]),
+        "one": (1024, None, [(1, 1025), (1, 1200), (1, 1400), (1, 1030)]),
+        "two_runs": (1056, [3, 1, 2], [(1, 1057), (1, 1180), (1, 1058), (1, 333 + 1056), (1, 1300), (1, 1090)]),
+        "tokens": (1024, None, [(3, 1100), (1, 1025), (2, 1026), (6, 1150)]),
         "wide": (1024, None, [(1, 1025 + 37 * i) for i in range(24)]),
-        "idle": (256, None, [(1, 300), (0, 300), (1, 512), (2, 301)]),
+        "idle": (1536, None, [(1, 1600), (0, 1600), (1, 1800), (2, 1601)]),
     }[what]
     print(f"[case] shared prefix {what} type {type_}", flush=True)
     b = Batch(lens, page, shared, runs, seed=5)
     k, v = values(b, kv, D, type_, 4, shared, runs)
     q = (2 * np.random.default_rng(6).standard_normal((b.T, H, D))).astype(np.float32)
+    ctx.profile(True)
     got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    joins, _ = ctx.profile_read("join")
+    ctx.profile(False)
+    assert joins == 1, "the prefix was not shared"             # shared and own keys are two parts at least
     check(got, *attend64(b, q, k, v, D ** -0.5))
 
 
@@ -151,7 +155,7 @@ def test_score_and_query_ranges(ctx, type_):
 def test_batch_sizes(ctx, what, type_):
     """Parts for the join kernel, more sequences than blocks, more tiles than the card holds blocks."""
     H, kv, D = 8, 1, 64
-    lens, shared = {"long": ([(1, 20011)], 0), "long_group": ([(1, 9100), (1, 9500)], 9088), "many": ([(1, 1 + 7 * i % 61) for i in range(300)], 0),
+    lens, shared = {"long": ([(1, 20011)], 0), "long_group": ([(1, 33800), (1, 34100), (1, 33801), (1, 33900)], 33792), "many": ([(1, 1 + 7 * i % 61) for i in range(300)], 0),
                     "more_tiles_than_blocks": ([(150, 150 + i % 5) for i in range(110)], 0)}[what]
     print(f"[case] {what}, type {type_}", flush=True)
     b = Batch(lens, 64, shared, seed=24)

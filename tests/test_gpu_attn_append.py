@@ -156,11 +156,11 @@ def test_graph_follows_the_batch(ctx, type_):
     """Append and attention captured once, replayed on other batches: eager calls' bits each time."""
     hip, vp = hip_lib(), ctypes.c_void_p
     H, kv, D, page = 32, 4, 128, 16
-    shared = Batch([(1, 400), (1, 500), (1, 470)], page, 320, seed=11)
+    shared = Batch([(1, 6500), (1, 6600), (1, 6470)], page, 6416, seed=11)        # 26 MB of keys and values saved
     batches = [Batch([(1, 300), (1, 17), (1, 600)], page, seed=12), Batch([(1, 301), (1, 18), (1, 601)], page, seed=12), shared,
                Batch([(20, 50), (1, 3), (0, 9)], page, seed=13), Batch([(0, 0), (0, 4)], page, seed=14), Batch([(2, 2000)], page, seed=15)]
     top = Batch([(1, 1)], page)
-    top.n_page, top.T, top.max_pages, top.q = max(b.n_page for b in batches), 32, 125, [0] * 3
+    top.n_page, top.T, top.max_pages, top.q = max(b.n_page for b in batches), 32, 420, [0] * 3
     pool = Pool(ctx, H, kv, D, type_, top, rope_base=1e4)
     rng = np.random.default_rng(16)
     pools = [rng.standard_normal((top.n_page, kv, page, D)).astype(dtype_of(type_)) for _ in range(2)]
