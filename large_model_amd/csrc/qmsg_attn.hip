@@ -478,8 +478,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
     using A = Att<TYPE, D>;
     constexpr int NT = 1;
     __shared__ __align__(16) float s_o[kFewWaves][16][D + 4];
-    __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16];
+    __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16], s_top[16];
     __shared__ int s_last;
+    static_assert(16 * (D / 4) <= 64 * kFewWaves, "a thread for each four results");
+    const int o_row = threadIdx.x / (D / 4), o_d = threadIdx.x % (D / 4) * 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
     const AttnHdr &h = header(a);
@@ -498,6 +500,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
         AttRaw<TYPE, D> raw;
         load_q<TYPE, D>(a.q + ((size_t)qt * a.heads + (size_t)(kvh * a.group + qr % a.group)) * D, g, raw);
         const int limit[NT] = { min(toks[qt].pos + 1, w.key1) };
+        const int o_r = w.row + min(o_row, w.rows - 1), o_tok = o_r / a.group, o_head = kvh * a.group + o_r % a.group;
+        const AttnTok o_tk = toks[o_tok];
         const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
         const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
         u32x4 kf[A::NK], vf[A::NV];
@@ -561,43 +565,32 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
                 if (s + 2 * kFewWaves < n_step) pages(s + 2 * kFewWaves);
             }
         }
+        /* the waves' results on the largest of their references, then summed: thread i takes four values of row i / (D / 4) */
+        const float l = row_sum(row[0].l), mine = l != l ? INFINITY : row[0].ref;
+        if (g == 0) s_m[wave][col] = mine;
         const bool wild = __syncthreads_or(bad != 0);
+        float m = s_m[0][col];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const float l = row_sum(row[n].l);
-            if (g == 0) {
-                s_m[wave][col] = l != l ? INFINITY : row[n].ref;
-                s_l[wave][col] = l;
+        for (int i = 1; i < kFewWaves; i++) m = fmaxf(m, s_m[i][col]);
+        const float f = mine == kLowest ? 0.0f : exp2_fast(mine - m);
+        if (g == 0) s_l[wave][col] = l * f;
+        if (wave == 0 && g == 0) s_top[col] = m;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) *(f32x4 *)&s_o[wave][col][16 * i + 4 * g] = row[0].o[i] * f;
+        __syncthreads();
+        if (o_row < min(16, w.rows)) {
+            float ll = 0.0f;
+            f32x4 o = { 0, 0, 0, 0 };
+#pragma unroll
+            for (int i = 0; i < kFewWaves; i++) {
+                ll += s_l[i][o_row];
+                o += *(const f32x4 *)&s_o[i][o_row][o_d];
             }
-            __syncthreads();
-            float m = s_m[0][col];
-#pragma unroll
-            for (int i = 1; i < kFewWaves; i++) m = fmaxf(m, s_m[i][col]);
-            const float mine = l != l ? INFINITY : row[n].ref;
-            const float f = mine == kLowest ? 0.0f : exp2_fast(mine - m);
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) *(f32x4 *)&s_o[wave][col][16 * i + 4 * g] = row[n].o[i] * f;
-            __syncthreads();
-            for (int e = threadIdx.x; e < 16 * (D / 4); e += 64 * kFewWaves) {
-                const int rr = e / (D / 4), d = e % (D / 4) * 4;
-                if (16 * n + rr >= w.rows) continue;
-                float mm = s_m[0][rr], ll = 0.0f;
-#pragma unroll
-                for (int i = 1; i < kFewWaves; i++) mm = fmaxf(mm, s_m[i][rr]);
-                f32x4 o = { 0, 0, 0, 0 };
-#pragma unroll
-                for (int i = 0; i < kFewWaves; i++) {
-                    const float mi = s_m[i][rr];
-                    ll += mi == kLowest ? 0.0f : exp2_fast(mi - mm) * s_l[i][rr];
-                    o += *(const f32x4 *)&s_o[i][rr][d];
-                }
-                const int r = w.row + 16 * n + rr, t = r / a.group;
-                if (__builtin_expect(wild, 0))
-                    o += wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, min(toks[t].pos + 1, w.key1), d);
-                put_row(a, toks[t], w, t, kvh * a.group + r % a.group, d, D, mm, ll, o, d == 0);
-            }
-            __syncthreads();
+            if (__builtin_expect(wild, 0))
+                o += wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, min(o_tk.pos + 1, w.key1), o_d);
+            put_row(a, o_tk, w, o_tok, o_head, o_d, D, s_top[o_row], ll, o, o_d == 0);
         }
+        __syncthreads();
         join_tile<D, 64 * kFewWaves>(a, toks, w, kvh, s_last);
     }
 }
