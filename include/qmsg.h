@@ -1,4 +1,5 @@
-/* qmsg.h - MI355X (gfx950) Qwen3-MoE expert-FFN layer behind a plain C ABI.
+/* qmsg.h - MI355X (gfx950) Qwen3-MoE layers behind a plain C ABI: the expert FFN, the trunk's products
+ * and the attention over a paged cache.
  *
  * Drop-in for the reference engine's MoE layer with resident experts:
  *   static int moe(QmsModel *m, int l, const float *xn, const float *h, int T, float *out)
@@ -278,7 +279,9 @@ int qmsg_sync(qmsg_ctx *ctx);
  * paged cache of keys and values, and causal attention over it with grouped heads. Activations are
  * fp32; sums, norms and the softmax are formed in fp32 (fp16 caches: products of the cached values
  * with queries and weights of 22 bits). The reference's sums run in another order: results agree to
- * rounding, not bit for bit.
+ * rounding, not bit for bit, and the same batch gives the same bits on every run. Values past the cache's
+ * type become infinities in it. A key or value that is not finite reaches only the tokens that see it: their
+ * results are not defined for a key (the whole head), not finite for a value (its element).
  *
  * Order of calls, per step: qmsg_attn_batch with the sequences' lengths and page tables, then for
  * each layer qmsg_attn_append_device and qmsg_attn_device. */
@@ -301,7 +304,7 @@ uint64_t qmsg_attn_cache_bytes(const qmsg_attn_cfg *cfg);
 
 /* A cache and what its calls need (plans, workspace), freed with the context; *id names it. d_k and d_v:
  * the caller's device memory for keys and values (qmsg_attn_cache_bytes each, 16-byte aligned,
- * several may share it), or both NULL: the context's. Pages of keys are [kv head][slot][D], pages
+ * several may share it, not overlapping each other), or both NULL: the context's. Pages of keys are [kv head][slot][D], pages
  * of values [kv head][D][slot], layer by layer. Slots that hold no token yet may hold anything. */
 int qmsg_attn_create(qmsg_ctx *ctx, const qmsg_attn_cfg *cfg, void *d_k, void *d_v, int *id);
 int qmsg_attn_cache(qmsg_ctx *ctx, int id, void **d_k, void **d_v);
@@ -316,7 +319,8 @@ int qmsg_attn_norms(qmsg_ctx *ctx, int id, int layer, const float *q_norm, const
  * changes: a page id outside the cache, a page that would take new tokens twice, or more than the maxima
  * is QMSG_E_INVALID, and the batch stays what it was. Not while the stream is capturing; calls
  * captured into a graph work on the batch that is set when the graph is replayed (replay on
- * qmsg_stream(ctx), or ordered with it). */
+ * qmsg_stream(ctx), or ordered with it: an attention's calls share one workspace), and their buffers must hold
+ * that batch's rows. */
 int qmsg_attn_batch(qmsg_ctx *ctx, int id, int n_seq, const int *q_len, const int *kv_len, const int32_t *pages, int stride);
 
 /* For the batch's T new tokens, all on device buffers (16-byte aligned): norm and rotate the query heads
@@ -341,7 +345,8 @@ int qmsg_attn_mats(qmsg_ctx *ctx, int id, int layer, const int *ids, const float
 int qmsg_attn_layer(qmsg_ctx *ctx, int id, int layer, float *d_h, float eps);
 
 /* The attention keys of read_cfg (src/model.c:278-310) of a qwen3moe file: n_head, n_head_kv, head_dim, n_layer,
- * rope_base and qk_norm = 1; the other fields stay as they are. */
+ * rope_base and qk_norm = 1; the other fields stay as they are. Files that rotate a part of the head or scale
+ * positions (rope.dimension_count, rope.scaling.type) are QMSG_E_UNSUPPORTED. */
 int qmsg_gguf_attn_cfg(const qmsg_gguf *g, qmsg_attn_cfg *cfg);
 /* The attention lines of qms_model_load for file layers first .. first+n-1 into the layers of the same index:
  * blk.L.attn_{q,k,v,output}.weight, attn_norm, attn_q_norm and attn_k_norm (F32; without qk_norm the last

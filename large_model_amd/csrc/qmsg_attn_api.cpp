@@ -12,9 +12,18 @@ using namespace qmsg;
 
 namespace {
 
+/* Bytes of a cache's keys that are taken: more than a card has, and layers of any page fit 64 bits below it. */
+constexpr uint64_t kMostBytes = 1ull << 48;
+
 uint64_t page_bytes_of(const qmsg_attn_cfg &f)
 {
     return (uint64_t)f.n_head_kv * (uint64_t)f.page_tokens * (uint64_t)f.head_dim * (f.type == QMSG_T_F16 ? 2 : 4);
+}
+
+/* The scores' scale for exponents of two. */
+float log2_scale(const qmsg_attn_cfg &f)
+{
+    return (float)((f.scale > 0.0f ? (double)f.scale : 1.0 / std::sqrt((double)f.head_dim)) * 1.4426950408889634);
 }
 
 /* Whether the kernels take this configuration; 0 and the reason otherwise. */
@@ -26,8 +35,8 @@ int check_cfg(const qmsg_attn_cfg &f, const char **why)
         *why = "bad shape";
         return QMSG_E_INVALID;
     }
-    if (!(f.rope_base > 0.0f) || !std::isfinite(f.rope_base) || !(f.scale >= 0.0f) || !std::isfinite(f.scale)) {
-        *why = "rope_base must be positive and scale not negative";
+    if (!(f.rope_base > 0.0f) || !std::isfinite(f.rope_base) || !(f.scale >= 0.0f) || (f.scale > 0.0f && !std::isfinite(log2_scale(f)))) {
+        *why = "rope_base must be positive and scale not negative, both finite";
         return QMSG_E_INVALID;
     }
     if (f.type != QMSG_T_F16 && f.type != QMSG_T_F32) *why = "cache types are F16 and F32";
@@ -38,6 +47,8 @@ int check_cfg(const qmsg_attn_cfg &f, const char **why)
              (int64_t)f.max_tokens * f.n_head > INT32_MAX)
         *why = "tokens of the pool, tokens of a sequence and rows of a batch are 32-bit";
     else if ((int64_t)f.max_seq * f.max_pages > 1 << 28) *why = "page tables above 2^28 pages";
+    else if (f.n_layer > 1 << 16) *why = "more than 65536 layers";
+    else if ((uint64_t)f.n_page * page_bytes_of(f) > kMostBytes / (uint64_t)f.n_layer) *why = "keys above 2^48 bytes";
     return *why ? QMSG_E_UNSUPPORTED : QMSG_OK;
 }
 
@@ -91,7 +102,7 @@ int make_call(qmsg_ctx *c, const AttnStore &a, int layer, AttnCall *o)
     k.heads = a.cfg.n_head;
     k.kv_heads = a.cfg.n_head_kv;
     k.group = a.cfg.n_head / a.cfg.n_head_kv;
-    k.scale_log2 = (float)((a.cfg.scale > 0.0f ? (double)a.cfg.scale : 1.0 / std::sqrt((double)a.cfg.head_dim)) * 1.4426950408889634);
+    k.scale_log2 = log2_scale(a.cfg);
     k.done = a.done;
     k.part_o = a.part_o;
     k.part_ml = a.part_ml;
@@ -185,6 +196,9 @@ int qmsg_attn_create(qmsg_ctx *c, const qmsg_attn_cfg *f, void *d_k, void *d_v, 
     if (attn_blob_bytes(shape_of(*f)) > INT32_MAX) return fail(c, QMSG_E_UNSUPPORTED, "qmsg_attn_create: batches above 2 GiB of plan");
     if (!d_k != !d_v) return fail(c, QMSG_E_INVALID, "qmsg_attn_create: give both of d_k and d_v, or neither");
     if (((uintptr_t)d_k | (uintptr_t)d_v) & 15) return fail(c, QMSG_E_INVALID, "qmsg_attn_create: d_k and d_v must be 16-byte aligned");
+    const uint64_t bytes = qmsg_attn_cache_bytes(f);
+    if (d_k && (uintptr_t)d_k < (uintptr_t)d_v + bytes && (uintptr_t)d_v < (uintptr_t)d_k + bytes)
+        return fail(c, QMSG_E_INVALID, "qmsg_attn_create: d_k and d_v overlap");
     HIP_TRY(c, hipSetDevice(c->device));
     NO_THROW(c, "qmsg_attn_create", {
         auto a = std::make_unique<AttnStore>();
@@ -402,6 +416,13 @@ int qmsg_gguf_attn_cfg(const qmsg_gguf *g, qmsg_attn_cfg *f)
     if (g->scalar("qwen3moe.attention.value_length") && (rc = qmsg_gguf_get_int(g, "qwen3moe.attention.value_length", &dv))) return rc;
     if (dk != dv || dk <= 0 || dk > 1 << 20)
         return fail(nullptr, QMSG_E_UNSUPPORTED, "qmsg_gguf_attn_cfg: key_length %lld, value_length %lld", (long long)dk, (long long)dv);
+    /* rotations that the kernels do not have: of a part of the head, at stretched positions */
+    int64_t n_rot = dk;
+    if (g->scalar("qwen3moe.rope.dimension_count") && (rc = qmsg_gguf_get_int(g, "qwen3moe.rope.dimension_count", &n_rot))) return rc;
+    if (n_rot != dk) return fail(nullptr, QMSG_E_UNSUPPORTED, "qmsg_gguf_attn_cfg: rope.dimension_count %lld of heads of %lld", (long long)n_rot, (long long)dk);
+    char how[16] = "none";
+    if (g->scalar("qwen3moe.rope.scaling.type") && (rc = qmsg_gguf_get_str(g, "qwen3moe.rope.scaling.type", how, sizeof how))) return rc;
+    if (strcmp(how, "none")) return fail(nullptr, QMSG_E_UNSUPPORTED, "qmsg_gguf_attn_cfg: rope.scaling.type %s", how);
     double base = 10000.0;
     if (g->scalar("qwen3moe.rope.freq_base") && (rc = qmsg_gguf_get_float(g, "qwen3moe.rope.freq_base", &base))) return rc;
     f->n_head = (int)v[0];

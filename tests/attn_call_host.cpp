@@ -160,6 +160,7 @@ static void configs()
     expect(QMSG_E_INVALID, [](qmsg_attn_cfg &f) { f.rope_base = INFINITY; });
     expect(QMSG_E_INVALID, [](qmsg_attn_cfg &f) { f.scale = -1.0f; });
     expect(QMSG_E_INVALID, [](qmsg_attn_cfg &f) { f.scale = NAN; });
+    expect(QMSG_E_INVALID, [](qmsg_attn_cfg &f) { f.scale = 3e38f; });          /* infinite in powers of two */
     expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) { f.type = QMSG_T_Q8_0; });
     for (int d : { 0, 32, 96, 256 }) expect(QMSG_E_UNSUPPORTED, [&](qmsg_attn_cfg &f) { f.head_dim = d; });
     for (int p : { 0, 8, 24, 512, -16 }) expect(QMSG_E_UNSUPPORTED, [&](qmsg_attn_cfg &f) { f.page_tokens = p; });
@@ -168,11 +169,25 @@ static void configs()
     expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) { f.max_pages = INT32_MAX; });
     expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) { f.max_tokens = INT32_MAX; });
     expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) { f.max_seq = f.max_pages = 1 << 26; });
+    expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) { f.n_layer = (1 << 16) + 1; });
+    expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) { f.n_layer = INT32_MAX; });
+    /* bytes that would wrap in 64 bits: 2^19 pages of 2^27 bytes, 2^16 layers and more */
+    expect(QMSG_E_UNSUPPORTED, [](qmsg_attn_cfg &f) {
+        f.n_head = f.n_head_kv = 1024;
+        f.type = QMSG_T_F32;
+        f.head_dim = 128;
+        f.page_tokens = 256;
+        f.n_page = 1 << 22;
+        f.n_layer = 1 << 16;
+    });
     qmsg_attn_cfg f = config();
+    CHECK(qmsg_attn_create(ctx, &f, kK, kK, &id) == QMSG_E_INVALID && qmsg_attn_create(ctx, &f, kK, (char *)kK + qmsg_attn_cache_bytes(&f) - 16, &id) == QMSG_E_INVALID);
+    CHECK(qmsg_attn_create(ctx, &f, (char *)kK + qmsg_attn_cache_bytes(&f) - 16, kK, &id) == QMSG_E_INVALID);
     CHECK(qmsg_attn_create(nullptr, &f, nullptr, nullptr, &id) == QMSG_E_INVALID && qmsg_attn_create(ctx, nullptr, nullptr, nullptr, &id) == QMSG_E_INVALID);
     CHECK(qmsg_attn_create(ctx, &f, kK, nullptr, &id) == QMSG_E_INVALID && qmsg_attn_create(ctx, &f, nullptr, kV, &id) == QMSG_E_INVALID);
     CHECK(qmsg_attn_create(ctx, &f, (char *)kK + 8, kV, &id) == QMSG_E_INVALID);
     CHECK(qmsg_attn_cache_bytes(&f) == 2ull * 32 * 2 * 16 * 64 * 2 && qmsg_attn_cache_bytes(nullptr) == 0);
+    CHECK(qmsg_attn_create(ctx, &f, kK, (char *)kK + qmsg_attn_cache_bytes(&f), &id) == QMSG_OK);
 }
 
 static void memory()

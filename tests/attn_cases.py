@@ -68,7 +68,7 @@ def attend64(batch, q, k, v, scale):
 
     With e = 2^-24, n keys, u_j = scale * sum_i |q_i k_ji|: a score's D products and its D + 8 roundings (the two halves of
     a split q included) move it by at most (D + 8) e u_j, taking it to powers of two and off the reference by 4 e (|s_j| +
-    max |s|) more; exp2 gives 2 steps, a p split into two truncated f16 leaves 2^-20 of it, and n sums in each of numerator
+    max |s|) more; exp2 gives 2 steps, a p split into two f16, each rounded to nearest, leaves 2^-22 of it (2^-20 allowed), and n sums in each of numerator
     and denominator 2 n e, a few more in joining parts. Relative to sum p |v| / sum p, first order, doubled for
     what products of these errors add."""
     T, H, D = q.shape

@@ -64,8 +64,11 @@ def test_gguf_attention_keys(tmp_path):
             return g.attn_cfg()
 
     assert cfg() == {"n_head": 8, "n_head_kv": 4, "head_dim": 64, "n_layer": 3, "rope_base": 10000.0}
+    same = {"rope__dimension_count": (U32, 64), "rope__scaling__type": (STR, "none")}
+    assert cfg(**same) == cfg()
     for change, status in (({"attention__head_count": None}, -1), ({"attention__head_count_kv": None}, -1), ({"attention__head_count": (U32, 0)}, -1),
-                           ({"attention__key_length": (U32, 64), "attention__value_length": (U32, 128)}, -2), ({"attention__key_length": (STR, "x")}, -1)):
+                           ({"attention__key_length": (U32, 64), "attention__value_length": (U32, 128)}, -2), ({"attention__key_length": (STR, "x")}, -1),
+                           ({"rope__dimension_count": (U32, 32)}, -2), ({"rope__scaling__type": (STR, "yarn")}, -2)):
         with pytest.raises(qmsg.QmsgError) as e:
             cfg(**change)
         assert e.value.status == status, change
