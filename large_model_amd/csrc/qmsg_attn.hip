@@ -159,31 +159,31 @@ __device__ __forceinline__ float make_q(AttRaw<TYPE, D> &raw, float scale, AttQ<
     }
 }
 
-/* A piece of keys (piece c of tile t) times NT rows, into their scores. */
-template <int TYPE, int D, int NT>
-__device__ __forceinline__ void score(u32x4 k, int c, int t, const AttQ<TYPE, D> (&q)[NT], f32x4 (&s)[NT][Att<TYPE, D>::TL])
+/* A piece of keys (piece c of tile t) times the first NA of a wave's NT row tiles, into their scores. */
+template <int TYPE, int D, int NT, int NA>
+__device__ __forceinline__ void score(u32x4 k, int c, int t, const AttQ<TYPE, D> (&q)[NT], f32x4 (&s)[NA][Att<TYPE, D>::TL])
 {
     if constexpr (TYPE == 0) {
         const f32x4 x = __builtin_bit_cast(f32x4, k);
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[n].v[c][e], s[n][t], 0, 0, 0);
+            for (int n = 0; n < NA; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[n].v[c][e], s[n][t], 0, 0, 0);
     } else {
         const h8 x = __builtin_bit_cast(h8, k);
 #pragma unroll
-        for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].lo[c], s[n][t], 0, 0, 0);
+        for (int n = 0; n < NA; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].lo[c], s[n][t], 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < NT; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].hi[c], s[n][t], 0, 0, 0);
+        for (int n = 0; n < NA; n++) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[n].hi[c], s[n][t], 0, 0, 0);
     }
 }
 
 /* A step's scores s[n][t][r] of key g * CE + 4 t + r start at `from`: they come out off their references. */
-template <int NT, int TL>
-__device__ __forceinline__ void score_from(const float (&from)[NT], f32x4 (&s)[NT][TL])
+template <int NT, int NA, int TL>
+__device__ __forceinline__ void score_from(const float (&from)[NT], f32x4 (&s)[NA][TL])
 {
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int n = 0; n < NA; n++)
 #pragma unroll
         for (int t = 0; t < TL; t++) s[n][t] = f32x4{ from[n], from[n], from[n], from[n] };
 }
@@ -199,11 +199,11 @@ struct AttP<0> {
 };
 
 /* Scores of rows whose query was scaled up, taken back down. */
-template <int NT, int NS, int TL>
-__device__ __forceinline__ void unscale(const float (&up)[NT], f32x4 (&s)[NS][NT][TL])
+template <int NT, int NA, int NS, int TL>
+__device__ __forceinline__ void unscale(const float (&up)[NT], f32x4 (&s)[NS][NA][TL])
 {
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+    for (int n = 0; n < NA; n++) {
         const float down = 1.0f / up[n];                     /* powers of two */
 #pragma unroll
         for (int k = 0; k < NS; k++)
@@ -222,15 +222,15 @@ __device__ __forceinline__ void hide(int left, f32x4 (&s)[TL])
         for (int r = 0; r < 4; r++) s[t][r] = 4 * t + r < left ? s[t][r] : kLowest;
 }
 
-/* Raise the references of NT row tiles for NS steps of scores (off their references) where one is too far
+/* Raise the references of NA row tiles for NS steps of scores (off their references) where one is too far
  * above its row's. */
-template <int D, int NT, int NS, int TL>
-__device__ __forceinline__ void raise(const float (&up)[NT], f32x4 (&s)[NS][NT][TL], float (&from)[NT], AttRow<D> (&row)[NT])
+template <int D, int NT, int NA, int NS, int TL>
+__device__ __forceinline__ void raise(const float (&up)[NT], f32x4 (&s)[NS][NA][TL], float (&from)[NT], AttRow<D> (&row)[NT])
 {
-    float top[NT];
+    float top[NA];
     bool far = false;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+    for (int n = 0; n < NA; n++) {
         top[n] = s[0][n][0][0];
 #pragma unroll
         for (int k = 0; k < NS; k++)
@@ -243,7 +243,7 @@ __device__ __forceinline__ void raise(const float (&up)[NT], f32x4 (&s)[NS][NT][
     }
     if (__builtin_expect(__ballot(far) != 0, 0)) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NA; n++) {
             const float base = row[n].ref == kLowest ? 0.0f : row[n].ref;
             const float ref = fmaxf(row[n].ref, base + row_max(top[n]) - 6.0f);
             const float a = ref == row[n].ref ? 1.0f : exp2_fast(row[n].ref - ref);
@@ -322,23 +322,23 @@ __device__ __forceinline__ u32x4 clean(u32x4 v, const AttMask &m, uint32_t &bad)
     return v;
 }
 
-/* O^T += V^T P^T of NT rows for the piece v of values d = 16 i + col. */
-template <int TYPE, int D, int NT>
-__device__ __forceinline__ void weigh(u32x4 v, int i, const AttP<TYPE> (&p)[NT], AttRow<D> (&row)[NT])
+/* O^T += V^T P^T of NA row tiles for the piece v of values d = 16 i + col. */
+template <int TYPE, int D, int NT, int NA>
+__device__ __forceinline__ void weigh(u32x4 v, int i, const AttP<TYPE> (&p)[NA], AttRow<D> (&row)[NT])
 {
     if constexpr (TYPE == 0) {
         const f32x4 x = __builtin_bit_cast(f32x4, v);
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[n].v[e], row[n].o[i], 0, 0, 0);
+            for (int n = 0; n < NA; n++) row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[n].v[e], row[n].o[i], 0, 0, 0);
     } else {
         const h8 x = __builtin_bit_cast(h8, v);
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NA; n++)
             row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, u32x4{ p[n].hi[0], p[n].hi[1], p[n].hi[2], p[n].hi[3] }), row[n].o[i], 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NA; n++)
             row[n].o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, u32x4{ p[n].lo[0], p[n].lo[1], p[n].lo[2], p[n].lo[3] }), row[n].o[i], 0, 0, 0);
     }
 }
@@ -545,7 +545,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 #pragma unroll
             for (int i = 0; i < A::NCH; i++)
 #pragma unroll
-                for (int t = 0; t < A::TL; t++) score<TYPE, D, NT>(kf[t * A::NCH + i], i, t, q, sc[0]);
+                for (int t = 0; t < A::TL; t++) score<TYPE, D>(kf[t * A::NCH + i], i, t, q, sc[0]);
             if (!unit) unscale(up, sc);
             if (more) load_k(s + kFewWaves);
             if (mask) {
@@ -559,7 +559,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 #pragma unroll
             for (int t = 0; t < A::TL; t++) soften<TYPE, D>(t, sc[0][0][t], row[0], p[0]);
 #pragma unroll
-            for (int i = 0; i < A::NV; i++) weigh<TYPE, D, NT>(vf[i], i, p, row);
+            for (int i = 0; i < A::NV; i++) weigh<TYPE, D>(vf[i], i, p, row);
             if (more) {
                 load_v(s + kFewWaves);
                 if (s + 2 * kFewWaves < n_step) pages(s + 2 * kFewWaves);
@@ -616,8 +616,9 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
     constexpr int RP = D * A::ES >= 256 ? 1 : 256 / (D * A::ES);    /* key rows per 256 bytes     */
     static_assert(VC == 8, "a row of values is 128 bytes");
     __shared__ __align__(16) uint8_t lds[2][2][L::BYTES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), P1 = (1 << a.shift) - 1;
+    /* the wave's row tiles are tile + 4 n; the first tile's place turns with the block, since the blocks 256 apart share a CU */
+    const int tile0 = (wave + (blockIdx.x >> 8) * 2) & 3;
     const AttnHdr &h = header(a);
     const int n_unit = h.n_run[kAttnMany] * a.kv_heads;
     const AttnWork *work = (const AttnWork *)(a.blob + h.work[kAttnMany]);
@@ -625,6 +626,9 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
     for (int u = blockIdx.x, next = -1; next >= 0 || u < n_unit;) {
         const AttnWork w = work[next >= 0 ? next : u / a.kv_heads];
         const int kvh = u % a.kv_heads;
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));                               /* an item's addresses are not kept for the next one */
+        const int lane = tid & 63, col = lane & 15, g = lane >> 4;
         next = w.next;
         if (next < 0) u += gridDim.x;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
@@ -633,7 +637,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
         int limit[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {                              /* rows behind the last one: its query, not stored */
-            const int r = w.row + min(16 * NT * wave + 16 * n + col, w.rows - 1), t = r / a.group;
+            const int r = w.row + min(16 * (tile0 + 4 * n) + col, w.rows - 1), t = r / a.group;
             load_q<TYPE, D>(a.q + ((size_t)t * a.heads + (size_t)(kvh * a.group + r % a.group)) * D, g, raw[n]);
             limit[n] = min(toks[t].pos + 1, w.key1);
         }
@@ -673,7 +677,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
             if (n_tile > 1) pages(1);
         }
         uint32_t bad = 0;
-        const bool idle = 16 * NT * wave >= w.rows;
+        const int n_own = (w.rows - 16 * tile0 + 63) / 64;          /* row tiles that hold rows */
         AttQ<TYPE, D> q[NT];
         AttRow<D> row[NT];
         float up[NT], from[NT] = {};
@@ -693,13 +697,13 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
         /* Steps of a tile, from st0 on: all their scores first, so that one branch serves them. LDS reads run two
          * pieces of keys and four of values ahead of their products, and a step's softmax between the
          * products of the one before; the barriers keep the compiler from undoing that. */
-        auto work_on = [&](auto masked, auto steps, int tile, int st0) {
+        auto work_on = [&](auto masked, auto steps, auto own, int tile, int st0) {
             constexpr bool MASK = decltype(masked)::value;
-            constexpr int NS = decltype(steps)::value, GK = NS * A::NCH, GV = NS * A::NV, KB = 3, VB = 4;
+            constexpr int NS = decltype(steps)::value, NA = decltype(own)::value, GK = NS * A::NCH, GV = NS * A::NV, KB = 3, VB = 4;
             const uint8_t *kr = lds[tile & 1][0] + (st0 * A::KS + (col >> 2) * A::CE + (col & 3)) * D * A::ES;
             const uint8_t *vr = lds[tile & 1][1] + col * 128;
             const int at = w.key0 + tile * L::KT + st0 * A::KS + g * A::CE;
-            f32x4 sc[NS][NT][A::TL];
+            f32x4 sc[NS][NA][A::TL];
             u32x4 kb[KB][A::TL], vb[VB];
             auto read_k = [&](int j) {
 #pragma unroll
@@ -707,8 +711,8 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
                     kb[j % KB][t] = *(const u32x4 *)(kr + (j / A::NCH * A::KS + 4 * t) * D * A::ES + (((4 * (j % A::NCH) + g) ^ (col / RP)) * 16));
             };
             auto read_v = [&](int j) { vb[j % VB] = *(const u32x4 *)(vr + 2048 * (j % A::NV) + (((4 * (st0 + j / A::NV) + g) ^ ((col >> 1) & 7)) * 16)); };
-            AttP<TYPE> p[2][NT];
-            constexpr int PARTS = NT * A::TL;                       /* of a step's softmax */
+            AttP<TYPE> p[2][NA];
+            constexpr int PARTS = NA * A::TL;                       /* of a step's softmax */
             auto soft = [&](int st, int k) { soften<TYPE, D>(k % A::TL, sc[st][k / A::TL][k % A::TL], row[k / A::TL], p[st % 2][k / A::TL]); };
             __builtin_amdgcn_s_setprio(1);                          /* over the SIMD's other wave where that has its softmax */
 #pragma unroll
@@ -720,7 +724,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
                 if (j + KB - 1 < GK) read_k(j + KB - 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int t = 0; t < A::TL; t++) score<TYPE, D, NT>(kb[j % KB][t], j % A::NCH, t, q, sc[j / A::NCH]);
+                for (int t = 0; t < A::TL; t++) score<TYPE, D>(kb[j % KB][t], j % A::NCH, t, q, sc[j / A::NCH]);
             }
 #pragma unroll
             for (int j = 0; j < VB; j++) read_v(j);
@@ -731,7 +735,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
 #pragma unroll
                 for (int st = 0; st < NS; st++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) hide(limit[n] - at - st * A::KS, sc[st][n]);
+                    for (int n = 0; n < NA; n++) hide(limit[n] - at - st * A::KS, sc[st][n]);
             }
             raise(up, sc, from, row);
 #pragma unroll
@@ -742,7 +746,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
                 const int st = j / A::NV, i = j % A::NV;
                 u32x4 v = vb[j % VB];
                 if constexpr (MASK) v = clean<TYPE>(v, piece_mask<TYPE>(w.full - at - st * A::KS, w.key1 - at - st * A::KS), bad);
-                weigh<TYPE, D, NT>(v, i, p[st % 2], row);
+                weigh<TYPE, D>(v, i, p[st % 2], row);
                 if (j + VB < GV) read_v(j + VB);
                 if (st + 1 < NS && i % (A::NV / PARTS) == 0) soft(st + 1, i / (A::NV / PARTS));
                 __builtin_amdgcn_sched_barrier(0);
@@ -750,22 +754,27 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
             __builtin_amdgcn_s_setprio(0);
         };
         const int n_clear = max(0, w.full - w.key0) / L::KT;        /* tiles that every row sees whole */
-        for (int tile = 0; tile < n_clear; tile++) {
-            turn(tile);
-            if (!idle) work_on(std::false_type{}, std::integral_constant<int, 2>{}, tile, 0);
-        }
+        /* each wave runs the loop of its own row tiles: the barriers in it are as many */
+        auto work_all = [&](auto own) {
+            for (int tile = 0; tile < n_clear; tile++) {
+                turn(tile);
+                if (n_own > 0) work_on(std::false_type{}, std::integral_constant<int, 2>{}, own, tile, 0);
+            }
 #pragma unroll 1
-        for (int tile = n_clear; tile < n_tile; tile++) {
-            turn(tile);
-            if (idle) continue;
+            for (int tile = n_clear; tile < n_tile; tile++) {
+                turn(tile);
+                if (n_own <= 0) continue;
 #pragma unroll 1
-            for (int st = 0; st < 2; st++)
-                if (w.key0 + tile * L::KT + st * A::KS < w.key1) work_on(std::true_type{}, std::integral_constant<int, 1>{}, tile, st);
-        }
+                for (int st = 0; st < 2; st++)
+                    if (w.key0 + tile * L::KT + st * A::KS < w.key1) work_on(std::true_type{}, std::integral_constant<int, 1>{}, own, tile, st);
+            }
+        };
+        if (NT == 1 || n_own >= NT) work_all(std::integral_constant<int, NT>{});
+        else work_all(std::integral_constant<int, 1>{});
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const float l = row_sum(row[n].l);
-            const int i = 16 * NT * wave + 16 * n + col, r = w.row + i, t = r / a.group, head = kvh * a.group + r % a.group;
+            const int i = 16 * (tile0 + 4 * n) + col, r = w.row + i, t = r / a.group, head = kvh * a.group + r % a.group;
             if (i >= w.rows) continue;
             const AttnTok tk = toks[t];
 #pragma unroll
@@ -786,15 +795,10 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
 
 /* Parts of a row joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. PL lanes of D / 4 threads take
  * every PL-th part in slot order, then lane 0 takes the lanes' results in theirs. */
-constexpr int kJoinLanes = 8;
-
 template <int D, int PL>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
+__device__ __forceinline__ void join_rows(const AttnCall &a, const AttnHdr &h, f32x4 (*s_o)[D / 4], float (*s_ml)[2])
 {
     constexpr int TPR = D / 4, RPB = 256 / (TPR * PL);
-    __shared__ __align__(16) f32x4 s_o[PL][RPB][TPR];
-    __shared__ float s_m[PL][RPB], s_l[PL][RPB];
-    const AttnHdr &h = header(a);
     const int n = h.n_comb * a.heads, d = threadIdx.x % TPR, pl = threadIdx.x / TPR % PL, rb = threadIdx.x / (TPR * PL);
     const int32_t *comb = (const int32_t *)(a.blob + h.comb);
     const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
@@ -803,27 +807,45 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
         const AttnTok tk = toks[t];
         const size_t r0 = (size_t)tk.part * a.heads + head;
         AttJoin j;
-        /* two parts' loads at a time */
-        for (int p = pl; p < tk.parts; p += 2 * PL) {
-            const size_t r = r0 + (size_t)p * a.heads, r2 = p + PL < tk.parts ? r + (size_t)PL * a.heads : r;
-            const float m1 = a.part_ml[2 * r], l1 = a.part_ml[2 * r + 1], m2 = a.part_ml[2 * r2], l2 = a.part_ml[2 * r2 + 1];
-            const f32x4 o1 = *(const f32x4 *)(a.part_o + r * D + 4 * d), o2 = *(const f32x4 *)(a.part_o + r2 * D + 4 * d);
-            j.add(m1, l1, o1);
-            if (r2 != r) j.add(m2, l2, o2);
+        for (int p = pl; p < tk.parts; p += 4 * PL) {               /* four parts' loads at a time */
+            f32x2 ml[4];
+            f32x4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const size_t r = r0 + (size_t)min(p + k * PL, tk.parts - 1) * a.heads;
+                ml[k] = *(const f32x2 *)(a.part_ml + 2 * r);
+                o[k] = *(const f32x4 *)(a.part_o + r * D + 4 * d);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (p + k * PL < tk.parts) j.add(ml[k].x, ml[k].y, o[k]);
         }
         if constexpr (PL > 1) {
-            s_o[pl][rb][d] = j.o;
+            s_o[rb * PL + pl][d] = j.o;
             if (d == 0) {
-                s_m[pl][rb] = j.m;
-                s_l[pl][rb] = j.l;
+                s_ml[rb * PL + pl][0] = j.m;
+                s_ml[rb * PL + pl][1] = j.l;
             }
             __syncthreads();
             if (pl == 0)
-                for (int k = 1; k < PL; k++) j.add(s_m[k][rb], s_l[k][rb], s_o[k][rb][d]);
+                for (int k = 1; k < PL; k++) j.add(s_ml[rb * PL + k][0], s_ml[rb * PL + k][1], s_o[rb * PL + k][d]);
             __syncthreads();
         }
         if (pl == 0 && i0 + rb < n) *(f32x4 *)(a.out + ((size_t)t * a.heads + head) * D + 4 * d) = j.o * (1.0f / j.l);
     }
+}
+
+constexpr int kJoinLanes = 8;
+__host__ __device__ inline int join_lanes(const AttnHdr &h) { return h.max_parts > 16 ? kJoinLanes : 1; }
+
+template <int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
+{
+    __shared__ __align__(16) f32x4 s_o[256 / (D / 4)][D / 4];
+    __shared__ float s_ml[256 / (D / 4)][2];
+    const AttnHdr &h = header(a);
+    if (join_lanes(h) > 1) join_rows<D, kJoinLanes>(a, h, s_o, s_ml);
+    else join_rows<D, 1>(a, h, s_o, s_ml);
 }
 
 /* Head norms, rotation and the append. Units of 16 (D 128) or 32 (D 64) heads of one token: D / 8 lanes a
@@ -925,11 +947,8 @@ hipError_t attend(const AttnCall &a, int grid, hipStream_t st)
     const int nb[kAttnKinds] = { a.live ? grid : a.h.n_run[0] * a.kv_heads, a.live ? grid : a.h.n_run[1] * a.kv_heads };
     if (nb[kAttnMany]) QLAUNCH("attend", (attn_many_kernel<TYPE, D>), dim3((unsigned)nb[kAttnMany]), dim3(kManyThreads), 0, st, a);
     if (nb[kAttnFew]) QLAUNCH("attend", (attn_few_kernel<TYPE, D>), dim3((unsigned)nb[kAttnFew]), dim3(64 * kFewWaves), 0, st, a);
-    /* rows of few parts a thread group each, others kJoinLanes groups */
-    const bool wide = a.live || a.h.max_parts > 4;
-    const int rpb = 256 / (D / 4 * (wide ? kJoinLanes : 1)), nj = a.live ? grid : (a.h.n_comb * a.heads + rpb - 1) / rpb;
-    if (nj && wide) QLAUNCH("join", (attn_join_kernel<D, kJoinLanes>), dim3((unsigned)nj), dim3(256), 0, st, a);
-    else if (nj) QLAUNCH("join", (attn_join_kernel<D, 1>), dim3((unsigned)nj), dim3(256), 0, st, a);
+    const int rpb = 256 / (D / 4 * join_lanes(a.h)), nj = a.live ? grid : (a.h.n_comb * a.heads + rpb - 1) / rpb;
+    if (nj) QLAUNCH("join", (attn_join_kernel<D>), dim3((unsigned)nj), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
