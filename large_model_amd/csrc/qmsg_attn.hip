@@ -469,7 +469,13 @@ __device__ __forceinline__ void join_tile(const AttnCall &a, const AttnTok *toks
 }
 
 /* Few rows (16): eight waves take every eighth step of the item's keys, each from memory straight
- * into the operands' registers with the next step's loads in flight, and join in LDS. */
+ * into the operands' registers with the next step's loads in flight, and join in LDS.
+ *
+ * Bound: the cache's bytes, read once; no byte is used twice in a block, so LDS would only add a step, and a
+ * wave's 16 loads of 16 bytes a lane in flight (one block of eight waves a CU) reach the rate of a large copy: 32
+ * sequences of 4096 to 8191 keys (64 heads on 4, f16) 54 us, 5.1 TB/s; one of 131071 keys 43 us, 6.2 TB/s,
+ * and 4 to join. Short calls are latency: a token over 513 keys 9.7 us, of which 3 pass until the first
+ * keys are there, 1 in the products, 5 in joining waves and items. */
 constexpr int kFewWaves = 8;
 
 template <int TYPE, int D>
@@ -595,9 +601,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
     }
 }
 
-/* Many rows (128): four waves of 32 rows each share tiles of keys and values, copied to LDS by the LDS
- * DMA, the next tile's copy in flight while one is worked on. Pieces are stored with their index in
- * the row xored by the row, so that the 16 rows a wave instruction reads lie in all banks. */
+/* Many rows (128, fp32 64): four waves of one or two row tiles of 16 share tiles of keys and values, copied to
+ * LDS by the LDS DMA, the next tile's copy in flight while one is worked on. Pieces are stored with their index in
+ * the row xored by the row, so that the 16 rows a wave instruction reads lie in all banks (no conflicts).
+ *
+ * Bound: the matrix cores. Two row tiles a wave halve its LDS reads per product; the two blocks that a CU
+ * holds have one wave each on a SIMD, one's softmax under the other's products. 2047 prompt tokens (64 heads on 4,
+ * f16): 119 us, 575 TFLOP/s of the formula, 1150 on the f16 pipe with both halves (a large library product: 1072);
+ * 509 tokens behind 16000: 202 us, 672 and 1344. The pipe is busy for two thirds of the cycles, at a clock that falls
+ * to 1.9 GHz under this load. 32x32 instructions are slower on data than these (a loop of nothing else: 1680
+ * against 1850 TFLOP/s). Up to 64 rows a wave has one row tile, since two waves with two leave two idle: 32
+ * sequences of 4 drafted tokens (64 rows) over 4007 keys 29 / 37 us. */
 constexpr int kManyThreads = 256;
 
 template <int TYPE, int D>
@@ -794,7 +808,9 @@ __global__ __launch_bounds__(kManyThreads, 2) void attn_many_kernel(AttnCall a)
 }
 
 /* Parts of a row joined: out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. PL lanes of D / 4 threads take
- * every PL-th part in slot order, then lane 0 takes the lanes' results in theirs. */
+ * every PL-th part in slot order, then lane 0 takes the lanes' results in theirs.
+ *
+ * Bound: latency, then the parts' bytes (16384 rows of 4 or 5 parts 7.8 us). */
 template <int D, int PL>
 __device__ __forceinline__ void join_rows(const AttnCall &a, const AttnHdr &h, f32x4 (*s_o)[D / 4], float (*s_ml)[2])
 {
@@ -835,6 +851,8 @@ __device__ __forceinline__ void join_rows(const AttnCall &a, const AttnHdr &h, f
     }
 }
 
+/* One lane up to 16 parts (four rounds of loads), else eight. us by one / eight lanes: 2560 rows of up to 11 parts 4.7 /
+ * 6.7; 64 rows of 63 parts 15.5 / 4.2, 256 of 79 19.0 / 5.2. */
 constexpr int kJoinLanes = 8;
 __host__ __device__ inline int join_lanes(const AttnHdr &h) { return h.max_parts > 16 ? kJoinLanes : 1; }
 
@@ -851,7 +869,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall a)
 /* Head norms, rotation and the append. Units of 16 (D 128) or 32 (D 64) heads of one token: D / 8 lanes a
  * head, each with four elements and their four partners half a head away, so that the norm's sum and
  * the rotation stay in the lanes. Values go through LDS in tiles of up to 32 tokens of one page, so that
- * their transposed rows are stored in runs. */
+ * their transposed rows are stored in runs.
+ *
+ * Bound: bytes for many tokens (2047 of 64 + 2 x 4 heads: 28 us, 5.2 TB/s, a large copy's rate), the launch for
+ * few (one token 2.8 us, 64 tokens 4.1). One launch for q, k and v: three would cost more than the work. */
 template <int TYPE, int D>
 __global__ __launch_bounds__(256) void attn_append_kernel(AttnAppend b)
 {

@@ -43,7 +43,7 @@ int kind_of(int rows) { return rows <= attn_rows(kAttnFew, 1) ? kAttnFew : kAttn
 
 /* Blocks that a CU holds, the fewest keys worth a block, and what an item costs besides its keys, in keys. us by
  * fewest keys: one token over 513 keys 3.9 at 256, 4.1 in one piece of 513 (alone 22 / 24); 8 sequences of 5
- * drafted tokens 16.7 at 256, 15.7 at 384, 15.0 at 512, 15.7 at 768 (attention alone 23.8, 21.2, 22.7, 28.9); three fp32 prompts
+ * drafted tokens 14.8 at 256, 13.0 at 384, 12.8 at 512, 14.4 at 768 (alone 40.8, 38.8, 42.6, 46.7); three fp32 prompts
  * to 701 tokens 26.2 at 64 and 128, 27.2 at 256. By an item's cost of 64 / 128 / 192 / 256 keys: 64 sequences on
  * 8192 shared keys 44.4 / 42.7 / 43.0 / 41.7, the fp32 prompts 17.9 / 18.2 / 17.3 / 17.5. */
 constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };

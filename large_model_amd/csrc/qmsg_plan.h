@@ -83,8 +83,8 @@ struct AttnPlan {
 };
 
 /* Sharing that saves fewer bytes than this is left: its parts need a launch of their own to be joined. us (alone,
- * host round trip included) by the MB saved, shared / not: 4.3 6.6 / 3.7 (25.7 / 20.1), 16.5 8.9 / 11.2 (32.3 / 26.3),
- * 25.2 8.0 / 9.3 (30.4 / 27.2), 32.4 7.4 / 10.5 (27.4 / 27.1). */
+ * host round trip included) by the MB saved, shared / not: 4.3 6.2 / 3.9 (25 / 22), 15.6 6.3 / 6.5 (26 / 23), 24.8 8.8 /
+ * 10.0 (34 / 25), 33.6 6.6 / 10.1 (26 / 27), 62.9 10.0 / 14.9 (35 / 29), 66.1 10.8 / 21.5 (32 / 36). */
 constexpr int64_t kMinSaved = 24 << 20;
 
 /* Plan n_seq sequences: q_len[i] new tokens, the last of kv_len[i] tokens, on pages
