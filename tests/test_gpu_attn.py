@@ -165,6 +165,29 @@ def test_batch_sizes(ctx, what, type_):
     check(got, *attend64(b, q, k, v, D ** -0.5))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("group", [1, 16])
+def test_every_number_of_row_tiles(ctx, group, type_, D):
+    """Tiles of 17 to 128 rows in steps of a row (group 1) or a row tile (group 16), whose waves have none, one or two of
+    them, and more blocks than a card's CUs; a value that only a tile's last rows see is infinite."""
+    print(f"[case] group {group} type {type_} D {D}", flush=True)
+    kv = 8
+    rows = range(17, 129, 3) if group == 1 else [2, 3, 4, 5, 6, 7, 8] * 5
+    b = Batch([(n, n + 50 + 7 * i) for i, n in enumerate(rows)], 32, seed=group + D)
+    k, v = values(b, kv, D, type_, 5)
+    v[3][-1, 2, 5] = np.inf
+    q = np.random.default_rng(6).standard_normal((b.T, group * kv, D)).astype(np.float32)
+    got = Pool(ctx, group * kv, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    with np.errstate(invalid="ignore"):
+        want, tol = attend64(b, q, k, v, D ** -0.5)
+    last = sum(b.q[:4]) - 1                                   # the only token that sees it
+    hit = np.zeros(want.shape, bool)
+    hit[last, 2 * group:3 * group, 5] = True
+    assert np.all(np.isposinf(want[hit])) and not np.any(np.isfinite(got[hit]))
+    check(np.where(hit, 0, got), np.where(hit, 0, want), np.where(hit, 0, tol))
+
+
 def test_scale_and_layers(ctx):
     H, kv, D = 8, 2, 128
     b = Batch([(1, 100), (4, 60)], 32, seed=14)
