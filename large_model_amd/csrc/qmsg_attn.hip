@@ -468,37 +468,40 @@ __device__ __forceinline__ void join_tile(const AttnCall &a, const AttnTok *toks
     }
 }
 
-/* Few rows (16): eight waves take every eighth step of the item's keys, each from memory straight
- * into the operands' registers with the next step's loads in flight, and join in LDS.
+/* Few rows (16): eight waves (of many short items: one, two or four) take turns at the steps of the item's keys, each
+ * from memory straight into the operands' registers with the next step's loads in flight, and join in LDS.
  *
  * Bound: the cache's bytes, read once; no byte is used twice in a block, so LDS would only add a step, and a
  * wave's 16 loads of 16 bytes a lane in flight (one block of eight waves a CU) reach the rate of a large copy: 32
  * sequences of 4096 to 8191 keys (64 heads on 4, f16) 54 us, 5.1 TB/s; one of 131071 keys 43 us, 6.2 TB/s,
  * and 4 to join. Short calls are latency: a token over 513 keys 9.7 us, of which 3 pass until the first
- * keys are there, 1 in the products, 5 in joining waves and items. */
-constexpr int kFewWaves = 8;
+ * keys are there, 1 in the products, 5 in joining waves and items. 256 sequences of up to 101 keys: 13 us. */
+template <int D>
+struct FewLds {
+    __align__(16) float o[kFewWaves][16][D + 4];
+    float m[kFewWaves][16], l[kFewWaves][16], top[kFewWaves][16];
+    int last;
+};
 
-template <int TYPE, int D>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
+/* The launch's items with W waves each: a block's waves are groups of W with an item of their own. */
+template <int TYPE, int D, int W>
+__device__ __forceinline__ void few_items(const AttnCall &a, const AttnHdr &h, FewLds<D> &lds)
 {
     using A = Att<TYPE, D>;
-    constexpr int NT = 1;
-    __shared__ __align__(16) float s_o[kFewWaves][16][D + 4];
-    __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16], s_top[16];
-    __shared__ int s_last;
-    static_assert(16 * (D / 4) <= 64 * kFewWaves, "a thread for each four results");
-    const int o_row = threadIdx.x / (D / 4), o_d = threadIdx.x % (D / 4) * 4;
+    constexpr int NT = 1, groups = kFewWaves / W, o_rows = 64 * W / (D / 4);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, P1 = (1 << a.shift) - 1;
-    const AttnHdr &h = header(a);
     const int n_unit = h.n_run[kAttnFew] * a.kv_heads;
+    const int group = wave / W, sub = wave % W;
+    const int o_row = threadIdx.x % (64 * W) / (D / 4), o_d = threadIdx.x % (D / 4) * 4;
     const AttnWork *work = (const AttnWork *)(a.blob + h.work[kAttnFew]);
     const AttnTok *toks = (const AttnTok *)(a.blob + h.tok);
-    for (int u = blockIdx.x, next = -1; next >= 0 || u < n_unit;) {
+    for (int u0 = blockIdx.x * groups, next = -1; next >= 0 || u0 < n_unit;) {
+        const int u = min(u0 + group, n_unit - 1);
         const AttnWork w = work[next >= 0 ? next : u / a.kv_heads];
-        const int kvh = u % a.kv_heads;
+        const int kvh = u % a.kv_heads, n_row = u0 + group < n_unit ? min(w.rows, 16) : 0;      /* 0: no item for the group */
         next = w.next;
-        if (next < 0) u += gridDim.x;
+        if (next < 0) u0 += gridDim.x * groups;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
         /* a row behind the last one takes the last one's query: its results are not stored */
@@ -506,9 +509,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
         AttRaw<TYPE, D> raw;
         load_q<TYPE, D>(a.q + ((size_t)qt * a.heads + (size_t)(kvh * a.group + qr % a.group)) * D, g, raw);
         const int limit[NT] = { min(toks[qt].pos + 1, w.key1) };
-        const int o_r = w.row + min(o_row, w.rows - 1), o_tok = o_r / a.group, o_head = kvh * a.group + o_r % a.group;
-        const AttnTok o_tk = toks[o_tok];
-        const int n_step = (w.key1 - w.key0 + A::KS - 1) / A::KS, last = w.key1 - 1;
+        const int o_r = w.row + min(o_row, w.rows - 1);
+        int o_tok = o_r / a.group, o_head = kvh * a.group + o_r % a.group;
+        AttnTok o_tk = toks[o_tok];
+        const int n_step = n_row ? (w.key1 - w.key0 + A::KS - 1) / A::KS : 0, last = w.key1 - 1;
         const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
         u32x4 kf[A::NK], vf[A::NV];
         int kp = 0, vp = 0;
@@ -533,19 +537,19 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 #pragma unroll
             for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(p + i * step);
         };
-        if (wave < n_step) {
-            pages(wave);
-            load_k(wave);
-            load_v(wave);
-            if (wave + kFewWaves < n_step) pages(wave + kFewWaves);
+        if (sub < n_step) {
+            pages(sub);
+            load_k(sub);
+            load_v(sub);
+            if (sub + W < n_step) pages(sub + W);
         }
         AttQ<TYPE, D> q[NT];
         AttRow<D> row[NT];
         float up[NT] = { make_q<TYPE, D>(raw, a.scale_log2, q[0]) }, from[NT] = {};
         const bool unit = __ballot(up[0] != 1.0f) == 0;
-        for (int s = wave; s < n_step; s += kFewWaves) {
+        for (int s = sub; s < n_step; s += W) {
             const int key = w.key0 + s * A::KS;
-            const bool more = s + kFewWaves < n_step, mask = key + A::KS > w.full;
+            const bool more = s + W < n_step, mask = key + A::KS > w.full;
             f32x4 sc[1][NT][A::TL];
             score_from(from, sc[0]);
 #pragma unroll
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 #pragma unroll
                 for (int t = 0; t < A::TL; t++) score<TYPE, D>(kf[t * A::NCH + i], i, t, q, sc[0]);
             if (!unit) unscale(up, sc);
-            if (more) load_k(s + kFewWaves);
+            if (more) load_k(s + W);
             if (mask) {
                 hide(limit[0] - key - v_off, sc[0][0]);
                 const AttMask m = piece_mask<TYPE>(w.full - key - v_off, w.key1 - key - v_off);
@@ -567,38 +571,56 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
 #pragma unroll
             for (int i = 0; i < A::NV; i++) weigh<TYPE, D>(vf[i], i, p, row);
             if (more) {
-                load_v(s + kFewWaves);
-                if (s + 2 * kFewWaves < n_step) pages(s + 2 * kFewWaves);
+                load_v(s + W);
+                if (s + 2 * W < n_step) pages(s + 2 * W);
             }
         }
-        /* the waves' results on the largest of their references, then summed: thread i takes four values of row i / (D / 4) */
+        /* the group's results on the largest of its references, then summed: four values of a row a thread */
         const float l = row_sum(row[0].l), mine = l != l ? INFINITY : row[0].ref;
-        if (g == 0) s_m[wave][col] = mine;
+        if (g == 0) lds.m[wave][col] = mine;
         const bool wild = __syncthreads_or(bad != 0);
-        float m = s_m[0][col];
-#pragma unroll
-        for (int i = 1; i < kFewWaves; i++) m = fmaxf(m, s_m[i][col]);
+        const int first = group * W;
+        float m = lds.m[first][col];
+        for (int i = 1; i < W; i++) m = fmaxf(m, lds.m[first + i][col]);
         const float f = mine == kLowest ? 0.0f : exp2_fast(mine - m);
-        if (g == 0) s_l[wave][col] = l * f;
-        if (wave == 0 && g == 0) s_top[col] = m;
+        if (g == 0) lds.l[wave][col] = l * f;
+        if (sub == 0 && g == 0) lds.top[group][col] = m;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) *(f32x4 *)&s_o[wave][col][16 * i + 4 * g] = row[0].o[i] * f;
+        for (int i = 0; i < D / 16; i++) *(f32x4 *)&lds.o[wave][col][16 * i + 4 * g] = row[0].o[i] * f;
         __syncthreads();
-        if (o_row < min(16, w.rows)) {
+        for (int rr = o_row; rr < n_row; rr += o_rows) {
+            if (rr != o_row) {
+                const int r = w.row + rr;
+                o_tok = r / a.group;
+                o_head = kvh * a.group + r % a.group;
+                o_tk = toks[o_tok];
+            }
             float ll = 0.0f;
             f32x4 o = { 0, 0, 0, 0 };
-#pragma unroll
-            for (int i = 0; i < kFewWaves; i++) {
-                ll += s_l[i][o_row];
-                o += *(const f32x4 *)&s_o[i][o_row][o_d];
+            for (int i = 0; i < W; i++) {
+                ll += lds.l[first + i][rr];
+                o += *(const f32x4 *)&lds.o[first + i][rr][o_d];
             }
             if (__builtin_expect(wild, 0))
                 o += wild_sum<TYPE, D>(a.v, tab, a.page_bytes, head_off, a.shift, w.full, min(o_tk.pos + 1, w.key1), o_d);
-            put_row(a, o_tk, w, o_tok, o_head, o_d, D, s_top[o_row], ll, o, o_d == 0);
+            put_row(a, o_tk, w, o_tok, o_head, o_d, D, lds.top[group][rr], ll, o, o_d == 0);
         }
         __syncthreads();
-        join_tile<D, 64 * kFewWaves>(a, toks, w, kvh, s_last);
+        join_tile<D, 64 * kFewWaves>(a, toks, w, kvh, lds.last);
     }
+}
+
+/* W 0: a captured call's, which reads how many when it runs. */
+template <int TYPE, int D, int W>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void attn_few_kernel(AttnCall a)
+{
+    __shared__ FewLds<D> lds;
+    const AttnHdr &h = header(a);
+    if constexpr (W > 0) few_items<TYPE, D, W>(a, h, lds);
+    else if (h.few_shift == 3) few_items<TYPE, D, 8>(a, h, lds);
+    else if (h.few_shift == 2) few_items<TYPE, D, 4>(a, h, lds);
+    else if (h.few_shift == 1) few_items<TYPE, D, 2>(a, h, lds);
+    else few_items<TYPE, D, 1>(a, h, lds);
 }
 
 /* Many rows (128, fp32 64): four waves of one or two row tiles of 16 share tiles of keys and values, copied to
@@ -965,9 +987,19 @@ __global__ __launch_bounds__(256) void attn_append_kernel(AttnAppend b)
 template <int TYPE, int D>
 hipError_t attend(const AttnCall &a, int grid, hipStream_t st)
 {
-    const int nb[kAttnKinds] = { a.live ? grid : a.h.n_run[0] * a.kv_heads, a.live ? grid : a.h.n_run[1] * a.kv_heads };
+    const int groups = kFewWaves >> a.h.few_shift;
+    const int nb[kAttnKinds] = { a.live ? grid : (a.h.n_run[0] * a.kv_heads + groups - 1) / groups, a.live ? grid : a.h.n_run[1] * a.kv_heads };
     if (nb[kAttnMany]) QLAUNCH("attend", (attn_many_kernel<TYPE, D>), dim3((unsigned)nb[kAttnMany]), dim3(kManyThreads), 0, st, a);
-    if (nb[kAttnFew]) QLAUNCH("attend", (attn_few_kernel<TYPE, D>), dim3((unsigned)nb[kAttnFew]), dim3(64 * kFewWaves), 0, st, a);
+    if (nb[kAttnFew]) {
+        auto few = [&](auto waves) {
+            QLAUNCH("attend", (attn_few_kernel<TYPE, D, decltype(waves)::value>), dim3((unsigned)nb[kAttnFew]), dim3(64 * kFewWaves), 0, st, a);
+        };
+        if (a.live) few(std::integral_constant<int, 0>{});
+        else if (a.h.few_shift == 3) few(std::integral_constant<int, 8>{});
+        else if (a.h.few_shift == 2) few(std::integral_constant<int, 4>{});
+        else if (a.h.few_shift == 1) few(std::integral_constant<int, 2>{});
+        else few(std::integral_constant<int, 1>{});
+    }
     const int rpb = 256 / (D / 4 * join_lanes(a.h)), nj = a.live ? grid : (a.h.n_comb * a.heads + rpb - 1) / rpb;
     if (nj) QLAUNCH("join", (attn_join_kernel<D>), dim3((unsigned)nj), dim3(256), 0, st, a);
     return hipGetLastError();

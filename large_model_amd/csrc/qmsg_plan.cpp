@@ -327,6 +327,23 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
         first.insert(first.end(), later.begin(), later.end());
     }
 
+    /* Waves of an item of few rows: the fewest whose longest item ends with the others. Fewer waves join less and have
+     * more steps to overlap; each holds one step's loads in flight whatever their number. us by 8 / 4 / 2 / 1 (one token
+     * each; 64 heads on 4, f16): 256 sequences of up to 101 keys 29 / 19 / 15 / 19, of 501 keys 67 / 54 / 50 / 67, 128 of up
+     * to 1501 41 / 45 / 71 / 115; 16 heads on 16: 256 of up to 101 keys 88 / 55 / 38 / 29. */
+    int few_shift = 3;
+    if (std::all_of(work[kAttnFew].begin(), work[kAttnFew].end(), [](const AttnWork &w) { return w.joins == 1 && w.next < 0; })) {
+        const int step = s.type == 1 ? 32 : 16;                /* keys that a wave takes at a time */
+        int64_t steps = 0, most = 0;
+        for (const AttnWork &w : work[kAttnFew]) {
+            const int64_t n = (w.key1 - w.key0 + step - 1) / step;
+            steps += n;
+            most = std::max(most, n);
+        }
+        const double each = (double)(steps * s.kv_heads) / (2.0 * kFewWaves * n_cu);
+        for (few_shift = 0; few_shift < 3 && (double)most > (2.0 * each + 1.5) * (1 << few_shift);) few_shift++;
+    }
+
     std::vector<int32_t> comb;
     for (int k = 0; k < (int)T; k++)
         if (tok[(size_t)k].parts > 1 && apart[(size_t)k]) comb.push_back(k);
@@ -341,6 +358,7 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
     h.n_tok = (int)T;
     h.n_vt = (int)vt.size();
     h.n_comb = (int)comb.size();
+    h.few_shift = few_shift;
     for (const AttnTok &k : tok) h.max_parts = std::max(h.max_parts, k.parts);
     h.tok = place(tok.size() * sizeof(AttnTok));
     h.vt = place(vt.size() * sizeof(AttnVTile));

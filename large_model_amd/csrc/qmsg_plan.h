@@ -47,9 +47,10 @@ struct AttnWork {
  * through LDS. */
 enum { kAttnFew = 0, kAttnMany = 1, kAttnKinds = 2 };
 constexpr int attn_rows(int kind, int type) { return kind == kAttnFew ? 16 : type == 0 ? 64 : 128; }
+constexpr int kFewWaves = 8;              /* waves of a few-row block */
 /* Where the parts of a batch sit in its blob (byte offsets) and how many there are. */
 struct AttnHdr {
-    int32_t n_tok, n_vt, n_comb, max_parts, n_run[kAttnKinds];
+    int32_t n_tok, n_vt, n_comb, max_parts, few_shift, n_run[kAttnKinds];      /* 1 << few_shift: waves of an item of few rows */
     int32_t tok, vt, comb, work[kAttnKinds], pages, bytes;
     /* run r of a kind starts with item r */
 };

@@ -78,6 +78,10 @@ static void check(const AttnShape &s, int n_seq, const std::vector<int> &q, cons
                 reached.push_back(i);
             }
         CHECK((int)reached.size() == n_item);
+        /* fewer waves an item only for items that are a run and a tile each */
+        CHECK(h.few_shift >= 0 && 1 << h.few_shift <= kFewWaves);
+        if (kind == kAttnFew && 1 << h.few_shift < kFewWaves)
+            for (int i : reached) CHECK(w[i].next < 0 && w[i].count < 0 && w[i].joins == 1);
         for (int i : reached) {
             CHECK(w[i].rows > 0 && w[i].rows <= attn_rows(kind, s.type) && w[i].row >= 0 && w[i].row + w[i].rows <= T * G);
             CHECK(w[i].key0 >= 0 && w[i].key0 % 16 == 0 && w[i].key1 >= w[i].key0 && w[i].full <= w[i].key1);
@@ -131,7 +135,7 @@ int main(int argc, char **argv)
 {
     std::mt19937 rng((unsigned)atoi(argc > 1 ? argv[1] : "0"));
     auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
-    int n_shared = 0;
+    int n_shared = 0, n_waves[4] = { 0, 0, 0, 0 };
     for (batch = 0; batch < atoi(argc > 2 ? argv[2] : "1"); batch++) {
         static const int kHeads[][2] = { { 1, 1 }, { 14, 2 }, { 16, 16 }, { 32, 4 }, { 64, 4 }, { 6, 2 } };
         const int *hd = kHeads[pick(0, 5)];
@@ -167,6 +171,7 @@ int main(int argc, char **argv)
         bool sh = false;
         check(s, n_seq, q, kv, pages, stride, p, &sh);
         n_shared += sh;
+        if (p.h.n_run[kAttnFew]) n_waves[p.h.few_shift]++;
         /* what is wrong with a batch leaves the plan as it was */
         const std::vector<uint8_t> before = p.blob;
         int seq_bad = -1;
@@ -200,6 +205,6 @@ int main(int argc, char **argv)
             }
         CHECK(attn_plan(s, 256, n_seq, q.data(), kv.data(), pages.data(), stride, &p).empty());
     }
-    printf("%d batches, %d with a shared prefix\n", batch, n_shared);
+    printf("%d batches, %d with a shared prefix, %d %d %d %d with items of 1 2 4 8 waves\n", batch, n_shared, n_waves[0], n_waves[1], n_waves[2], n_waves[3]);
     return 0;
 }

@@ -23,4 +23,6 @@ def exe(tmp_path_factory):
 def test_random_batches(exe, seed):
     r = subprocess.run([exe, str(seed), "300"], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stderr[-2000:]
-    assert int(r.stdout.split()[2]) > 0, "no batch shared a prefix"
+    n = [int(x) for x in r.stdout.replace(",", "").split() if x.isdigit()]
+    assert n[1] > 0, "no batch shared a prefix"
+    assert all(n[2:6]), "no batch with items of some number of waves"

@@ -188,6 +188,30 @@ def test_every_number_of_row_tiles(ctx, group, type_, D):
     check(np.where(hit, 0, got), np.where(hit, 0, want), np.where(hit, 0, tol))
 
 
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads", [(16, 16, 128), (32, 4, 128), (14, 2, 64), (10, 2, 128)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("lens", ["ones", "steps", "ragged", "one_long", "odd"])
+def test_many_short_sequences(ctx, lens, heads, type_):
+    """Batches whose items have a wave or two each: as many as fill the card, an odd one at the end, some
+    sequences without new tokens, values that a draft's first token does not see."""
+    H, kv, D = heads
+    print(f"[case] {lens} {heads} type {type_}", flush=True)
+    n = [(1, 1)] * 150 if lens == "ones" else [(1, 1 + i % 70) for i in range(257)] if lens == "steps" else \
+        [(1 - (i % 9 == 4), 1 + 37 * i % 230) for i in range(300)] if lens == "ragged" else \
+        [(1, 60)] * 200 + [(1, 1500)] if lens == "one_long" else [(1 + (i % 3 == 0), 2 + 11 * i % 95) for i in range(131)]
+    b = Batch(n, 16, seed=len(n) + D)
+    k, v = values(b, kv, D, type_, 7)
+    for i in range(0, len(n), 7):
+        if b.q[i] == 2: v[i][-1, 0, 1] = -np.inf                  # its first token does not see this one
+    q = np.random.default_rng(8).standard_normal((b.T, H, D)).astype(np.float32)
+    got = Pool(ctx, H, kv, D, type_, b).run(q, *pack(b, k, v, kv, D, type_))
+    with np.errstate(invalid="ignore"):
+        want, tol = attend64(b, q, k, v, D ** -0.5)
+    hit = ~np.isfinite(want)
+    assert not np.any(np.isfinite(got[hit])) and (lens != "odd" or np.any(hit))
+    check(np.where(hit, 0, got), np.where(hit, 0, want), np.where(hit, 0, tol))
+
+
 def test_scale_and_layers(ctx):
     H, kv, D = 8, 2, 128
     b = Batch([(1, 100), (4, 60)], 32, seed=14)

@@ -204,6 +204,48 @@ def test_graph_follows_the_batch(ctx, type_):
         hip.hipGraphDestroy(graph)
 
 
+@pytest.mark.parametrize("type_", [F16, F32])
+def test_graph_of_few_and_many_sequences(ctx, type_):
+    """An attention captured once: batches whose items have one to eight waves, joined or not, long after short."""
+    hip, vp = hip_lib(), ctypes.c_void_p
+    H, kv, D, page = 16, 16, 128, 16
+    batches = [Batch([(1, 700), (1, 33)], page, seed=31), Batch([(1, 20)] * 260, page, seed=32), Batch([(1, 1 + i % 90) for i in range(259)], page, seed=33),
+               Batch([(1, 130)] * 40, page, seed=34), Batch([(1, 3000)], page, seed=35), Batch([(1, 5)] * 3, page, seed=36)]
+    top = Batch([(1, 1)] * 260, page)
+    top.n_page, top.max_pages = max(b.n_page for b in batches), 190
+    pool = Pool(ctx, H, kv, D, type_, top)
+    rng = np.random.default_rng(37)
+    for d in (pool.k, pool.v):
+        ctx.h2d(d, rng.standard_normal((top.n_page, kv, page, D)).astype(dtype_of(type_)))
+    r = Rows(ctx, 260, H, kv, D, 38)
+    d_o = ctx.device_alloc(r.q.nbytes)
+    st, graph, exe = vp(ctx_stream(ctx)), vp(), vp()
+
+    def result(run):
+        ctx.h2d(d_o, np.full(r.q.shape, 5.0, np.float32))
+        run()
+        ctx.sync()
+        return ctx.d2h(d_o, r.q.shape)
+
+    attend = lambda: ctx.attn_device(pool.id, 0, r.d[0], d_o)
+    ctx.attn_batch(pool.id, batches[0].q, batches[0].kv, batches[0].pages)
+    assert hip.hipStreamBeginCapture(st, 2) == 0
+    attend()
+    assert hip.hipStreamEndCapture(st, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, 0) == 0
+    try:
+        for n, b in enumerate(batches + batches[::-1]):
+            print(f"[case] batch {n}", flush=True)
+            ctx.attn_batch(pool.id, b.q, b.kv, b.pages)
+            want = result(attend)
+            assert np.all(want[b.T:] == 5.0)
+            for _ in range(2):
+                assert np.array_equal(result(lambda: hip.hipGraphLaunch(exe, st)), want), n
+    finally:
+        hip.hipGraphExecDestroy(exe)
+        hip.hipGraphDestroy(graph)
+
+
 def ctx_stream(ctx):
     from large_model_amd import qmsg
     return qmsg.lib.qmsg_stream(ctx._h)
