@@ -474,8 +474,9 @@ __device__ __forceinline__ void join_tile(const AttnCall &a, const AttnTok *toks
  * Bound: the cache's bytes, read once; no byte is used twice in a block, so LDS would only add a step, and a
  * wave's 16 loads of 16 bytes a lane in flight (one block of eight waves a CU) reach the rate of a large copy: 32
  * sequences of 4096 to 8191 keys (64 heads on 4, f16) 54 us, 5.1 TB/s; one of 131071 keys 43 us, 6.2 TB/s,
- * and 4 to join. Short calls are latency: a token over 513 keys 9.7 us, of which 3 pass until the first
- * keys are there, 1 in the products, 5 in joining waves and items. 256 sequences of up to 101 keys: 13 us. */
+ * and 4 to join. Short calls are latency: a token over 513 keys 9 us, of which 3 pass until the first
+ * keys' loads are issued, 2 until the products are done and 3 in joining waves and items; 2 sequences of 33 keys 6. Waves
+ * without a step load and join nothing (those 2 sequences 11 us otherwise). 256 sequences of up to 101 keys: 14 us. */
 template <int D>
 struct FewLds {
     __align__(16) float o[kFewWaves][16][D + 4];
@@ -504,89 +505,94 @@ __device__ __forceinline__ void few_items(const AttnCall &a, const AttnHdr &h, F
         if (next < 0) u0 += gridDim.x * groups;
         const int32_t *tab = (const int32_t *)(a.blob + h.pages) + w.pages;
         const uint32_t head_off = (uint32_t)kvh * ((uint32_t)(D * A::ES) << a.shift);
-        /* a row behind the last one takes the last one's query: its results are not stored */
-        const int qr = w.row + min(col, w.rows - 1), qt = qr / a.group;
-        AttRaw<TYPE, D> raw;
-        load_q<TYPE, D>(a.q + ((size_t)qt * a.heads + (size_t)(kvh * a.group + qr % a.group)) * D, g, raw);
-        const int limit[NT] = { min(toks[qt].pos + 1, w.key1) };
+        const int n_step = n_row ? (w.key1 - w.key0 + A::KS - 1) / A::KS : 0, busy = min(W, n_step);     /* waves with a step */
         const int o_r = w.row + min(o_row, w.rows - 1);
         int o_tok = o_r / a.group, o_head = kvh * a.group + o_r % a.group;
         AttnTok o_tk = toks[o_tok];
-        const int n_step = n_row ? (w.key1 - w.key0 + A::KS - 1) / A::KS : 0, last = w.key1 - 1;
-        const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
-        u32x4 kf[A::NK], vf[A::NV];
-        int kp = 0, vp = 0;
+        AttRow<D> row[NT];
         uint32_t bad = 0;
-        auto pages = [&](int s) {
-            const int k = w.key0 + s * A::KS;
-            kp = tab[min(k + k_off, last) >> a.shift];
-            vp = tab[min(k + v_off, last) >> a.shift];
-        };
-        auto load_k = [&](int s) {
-            const int slot = (w.key0 + s * A::KS + k_off) & P1;
-            const uint8_t *p = page_at(a.k, kp, a.page_bytes, head_off) + (uint32_t)(slot * D + g * A::CE) * A::ES;
+        if (sub < busy) {
+            /* a row behind the last one takes the last one's query: its results are not stored */
+            const int qr = w.row + min(col, w.rows - 1), qt = qr / a.group;
+            AttRaw<TYPE, D> raw;
+            load_q<TYPE, D>(a.q + ((size_t)qt * a.heads + (size_t)(kvh * a.group + qr % a.group)) * D, g, raw);
+            const int limit[NT] = { min(toks[qt].pos + 1, w.key1) };
+            const int last = w.key1 - 1;
+            const int k_off = (col >> 2) * A::CE + (col & 3), v_off = g * A::CE;
+            u32x4 kf[A::NK], vf[A::NV];
+            int kp = 0, vp = 0;
+            auto pages = [&](int s) {
+                const int k = w.key0 + s * A::KS;
+                kp = tab[min(k + k_off, last) >> a.shift];
+                vp = tab[min(k + v_off, last) >> a.shift];
+            };
+            auto load_k = [&](int s) {
+                const int slot = (w.key0 + s * A::KS + k_off) & P1;
+                const uint8_t *p = page_at(a.k, kp, a.page_bytes, head_off) + (uint32_t)(slot * D + g * A::CE) * A::ES;
 #pragma unroll
-            for (int t = 0; t < A::TL; t++)
+                for (int t = 0; t < A::TL; t++)
 #pragma unroll
-                for (int i = 0; i < A::NCH; i++) kf[t * A::NCH + i] = *(const u32x4 *)(p + (4 * t * D + 4 * i * A::CE) * A::ES);
-        };
-        auto load_v = [&](int s) {
-            const int slot = (w.key0 + s * A::KS + v_off) & P1;
-            const uint8_t *p = page_at(a.v, vp, a.page_bytes, head_off) + (uint32_t)((col << a.shift) + slot) * A::ES;
-            const uint32_t step = (uint32_t)(16 * A::ES) << a.shift;
+                    for (int i = 0; i < A::NCH; i++) kf[t * A::NCH + i] = *(const u32x4 *)(p + (4 * t * D + 4 * i * A::CE) * A::ES);
+            };
+            auto load_v = [&](int s) {
+                const int slot = (w.key0 + s * A::KS + v_off) & P1;
+                const uint8_t *p = page_at(a.v, vp, a.page_bytes, head_off) + (uint32_t)((col << a.shift) + slot) * A::ES;
+                const uint32_t step = (uint32_t)(16 * A::ES) << a.shift;
 #pragma unroll
-            for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(p + i * step);
-        };
-        if (sub < n_step) {
+                for (int i = 0; i < A::NV; i++) vf[i] = *(const u32x4 *)(p + i * step);
+            };
             pages(sub);
             load_k(sub);
             load_v(sub);
             if (sub + W < n_step) pages(sub + W);
-        }
-        AttQ<TYPE, D> q[NT];
-        AttRow<D> row[NT];
-        float up[NT] = { make_q<TYPE, D>(raw, a.scale_log2, q[0]) }, from[NT] = {};
-        const bool unit = __ballot(up[0] != 1.0f) == 0;
-        for (int s = sub; s < n_step; s += W) {
-            const int key = w.key0 + s * A::KS;
-            const bool more = s + W < n_step, mask = key + A::KS > w.full;
-            f32x4 sc[1][NT][A::TL];
-            score_from(from, sc[0]);
+            AttQ<TYPE, D> q[NT];
+            float up[NT] = { make_q<TYPE, D>(raw, a.scale_log2, q[0]) }, from[NT] = {};
+            const bool unit = __ballot(up[0] != 1.0f) == 0;
+            for (int s = sub; s < n_step; s += W) {
+                const int key = w.key0 + s * A::KS;
+                const bool more = s + W < n_step, mask = key + A::KS > w.full;
+                f32x4 sc[1][NT][A::TL];
+                score_from(from, sc[0]);
 #pragma unroll
-            for (int i = 0; i < A::NCH; i++)
+                for (int i = 0; i < A::NCH; i++)
 #pragma unroll
-                for (int t = 0; t < A::TL; t++) score<TYPE, D>(kf[t * A::NCH + i], i, t, q, sc[0]);
-            if (!unit) unscale(up, sc);
-            if (more) load_k(s + W);
-            if (mask) {
-                hide(limit[0] - key - v_off, sc[0][0]);
-                const AttMask m = piece_mask<TYPE>(w.full - key - v_off, w.key1 - key - v_off);
+                    for (int t = 0; t < A::TL; t++) score<TYPE, D>(kf[t * A::NCH + i], i, t, q, sc[0]);
+                if (!unit) unscale(up, sc);
+                if (more) load_k(s + W);
+                if (mask) {
+                    hide(limit[0] - key - v_off, sc[0][0]);
+                    const AttMask m = piece_mask<TYPE>(w.full - key - v_off, w.key1 - key - v_off);
 #pragma unroll
-                for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
-            }
-            raise(up, sc, from, row);
-            AttP<TYPE> p[NT];
+                    for (int i = 0; i < A::NV; i++) vf[i] = clean<TYPE>(vf[i], m, bad);
+                }
+                raise(up, sc, from, row);
+                AttP<TYPE> p[NT];
 #pragma unroll
-            for (int t = 0; t < A::TL; t++) soften<TYPE, D>(t, sc[0][0][t], row[0], p[0]);
+                for (int t = 0; t < A::TL; t++) soften<TYPE, D>(t, sc[0][0][t], row[0], p[0]);
 #pragma unroll
-            for (int i = 0; i < A::NV; i++) weigh<TYPE, D>(vf[i], i, p, row);
-            if (more) {
-                load_v(s + W);
-                if (s + 2 * W < n_step) pages(s + 2 * W);
+                for (int i = 0; i < A::NV; i++) weigh<TYPE, D>(vf[i], i, p, row);
+                if (more) {
+                    load_v(s + W);
+                    if (s + 2 * W < n_step) pages(s + 2 * W);
+                }
             }
         }
         /* the group's results on the largest of its references, then summed: four values of a row a thread */
         const float l = row_sum(row[0].l), mine = l != l ? INFINITY : row[0].ref;
-        if (g == 0) lds.m[wave][col] = mine;
+        if (g == 0 && sub < busy) lds.m[wave][col] = mine;
         const bool wild = __syncthreads_or(bad != 0);
         const int first = group * W;
-        float m = lds.m[first][col];
-        for (int i = 1; i < W; i++) m = fmaxf(m, lds.m[first + i][col]);
-        const float f = mine == kLowest ? 0.0f : exp2_fast(mine - m);
-        if (g == 0) lds.l[wave][col] = l * f;
-        if (sub == 0 && g == 0) lds.top[group][col] = m;
+        float m = kLowest;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) *(f32x4 *)&lds.o[wave][col][16 * i + 4 * g] = row[0].o[i] * f;
+        for (int i = 0; i < W; i++)
+            if (i < busy) m = fmaxf(m, lds.m[first + i][col]);
+        if (sub < busy) {
+            const float f = mine == kLowest ? 0.0f : exp2_fast(mine - m);
+            if (g == 0) lds.l[wave][col] = l * f;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) *(f32x4 *)&lds.o[wave][col][16 * i + 4 * g] = row[0].o[i] * f;
+        }
+        if (sub == 0 && g == 0) lds.top[group][col] = m;
         __syncthreads();
         for (int rr = o_row; rr < n_row; rr += o_rows) {
             if (rr != o_row) {
@@ -597,7 +603,9 @@ __device__ __forceinline__ void few_items(const AttnCall &a, const AttnHdr &h, F
             }
             float ll = 0.0f;
             f32x4 o = { 0, 0, 0, 0 };
+#pragma unroll
             for (int i = 0; i < W; i++) {
+                if (i >= busy) continue;
                 ll += lds.l[first + i][rr];
                 o += *(const f32x4 *)&lds.o[first + i][rr][o_d];
             }

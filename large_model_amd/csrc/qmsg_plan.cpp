@@ -327,10 +327,11 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
         first.insert(first.end(), later.begin(), later.end());
     }
 
-    /* Waves of an item of few rows: the fewest whose longest item ends with the others. Fewer waves join less and have
-     * more steps to overlap; each holds one step's loads in flight whatever their number. us by 8 / 4 / 2 / 1 (one token
-     * each; 64 heads on 4, f16): 256 sequences of up to 101 keys 29 / 19 / 15 / 19, of 501 keys 67 / 54 / 50 / 67, 128 of up
-     * to 1501 41 / 45 / 71 / 115; 16 heads on 16: 256 of up to 101 keys 88 / 55 / 38 / 29. */
+    /* Waves of an item of few rows: the fewest that leave a block for each CU and whose longest item ends with the others.
+     * Fewer waves join less and have more steps to overlap; each holds one step's loads in flight whatever their number.
+     * us by 8 / 4 / 2 / 1 (one token each; 64 heads on 4, f16): 256 sequences of up to 101 keys 29 / 19 / 15 / 19, of
+     * 501 keys 67 / 54 / 50 / 67, 128 of up to 101 15 / 10 / 13 / 18, of up to 1501 41 / 45 / 71 / 115; 16 heads on
+     * 16: 256 of up to 101 keys 88 / 55 / 38 / 29. */
     int few_shift = 3;
     if (std::all_of(work[kAttnFew].begin(), work[kAttnFew].end(), [](const AttnWork &w) { return w.joins == 1 && w.next < 0; })) {
         const int step = s.type == 1 ? 32 : 16;                /* keys that a wave takes at a time */
@@ -341,7 +342,8 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
             most = std::max(most, n);
         }
         const double each = (double)(steps * s.kv_heads) / (2.0 * kFewWaves * n_cu);
-        for (few_shift = 0; few_shift < 3 && (double)most > (2.0 * each + 1.5) * (1 << few_shift);) few_shift++;
+        const int64_t units = (int64_t)work[kAttnFew].size() * s.kv_heads;
+        for (few_shift = 0; few_shift < 3 && ((units << few_shift) < (int64_t)kFewWaves * n_cu || (double)most > (2.0 * each + 1.5) * (1 << few_shift));) few_shift++;
     }
 
     std::vector<int32_t> comb;
