@@ -44,11 +44,13 @@ int kind_of(int rows) { return rows <= attn_rows(kAttnFew, 1) ? kAttnFew : kAttn
 /* Blocks that a CU holds, the fewest keys worth a block, and what an item costs besides its keys, in keys. us by
  * fewest keys: one token over 513 keys 3.9 at 256, 4.1 in one piece of 513 (alone 22 / 24); 8 sequences of 5
  * drafted tokens 14.8 at 256, 13.0 at 384, 12.8 at 512, 14.4 at 768 (alone 40.8, 38.8, 42.6, 46.7); three fp32 prompts
- * to 701 tokens 26.2 at 64 and 128, 27.2 at 256. By an item's cost of 64 / 128 / 192 / 256 keys: 64 sequences on
- * 8192 shared keys 44.4 / 42.7 / 43.0 / 41.7, the fp32 prompts 17.9 / 18.2 / 17.3 / 17.5. */
+ * to 701 tokens 26.2 at 64 and 128, 27.2 at 256. By an item's cost of 192 / 256 / 320 / 384 keys (alone, the kernels):
+ * two prompts to 733 tokens, 64 heads on 4, 34.0 / 32.0 / 28.7 / 26.5 (54 / 57 / 58 / 48), 756 tokens behind 214
+ * 42.0 / 40.7 / 37.9 / 39.0 (63 / 62 / 57 / 57), 64 sequences on 8192 shared keys 44.6 / 43.4 / 42.9 / 46.2 (63 / 65
+ * / 65 / 69); fp32 prompts 17.9 at 64, 18.2 at 128, 17.3 at 192, 17.5 at 256. */
 constexpr int kBlocksPerCu[kAttnKinds] = { 1, 2 };
 constexpr int kMinKeys[kAttnKinds] = { 256, 384 }, kMinKeysF32 = 128;
-constexpr int kItemCost[kAttnKinds] = { 128, 192 };
+constexpr int kItemCost[kAttnKinds] = { 128, 320 }, kItemCostF32 = 192;
 /* Cuts fall on multiples of this many keys from a tile's first. */
 constexpr int kCut = 64;
 
@@ -191,6 +193,8 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
      * is nearly as even as equal shares of all tiles one after the other, whose runs may span tiles and whose tiles
      * come in more parts. `coarser`: runs that much longer, for fewer parts. */
     auto cut_tiles = [&](int kind, int64_t coarser) {
+        const bool f32 = kind == kAttnMany && s.type == 0;
+        const int64_t floor = f32 ? kMinKeysF32 : kMinKeys[kind], item = f32 ? kItemCostF32 : kItemCost[kind];
         std::vector<Tile *> of;
         int64_t cost = 0;
         for (Tile &x : tiles)
@@ -198,11 +202,10 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
                 of.push_back(&x);
                 x.cut.clear();
                 x.fresh = true;
-                cost += x.key1 - x.key0 + kItemCost[kind];
+                cost += x.key1 - x.key0 + item;
             }
         const int64_t slots = std::max<int64_t>(1, (int64_t)kBlocksPerCu[kind] * n_cu / s.kv_heads);
         if (of.empty() || (int64_t)of.size() >= 2 * slots) return;
-        const int64_t floor = kind == kAttnMany && s.type == 0 ? kMinKeysF32 : kMinKeys[kind];
         /* the shortest pieces of which there are no more than slots */
         int64_t piece = std::max((cost / slots + kCut - 1) / kCut * kCut, floor) * coarser, n_run = slots + 1;
         for (; (int64_t)of.size() <= slots; piece += piece / 64 / kCut * kCut + kCut) {
@@ -210,8 +213,8 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
             for (const Tile *x : of) n_run += (x->key1 - x->key0 + piece - 1) / piece;
             if (n_run <= slots) break;
         }
-        int64_t share = std::max(cost / slots, floor) * coarser + kItemCost[kind];
-        if (n_run <= slots && piece + kItemCost[kind] <= share + share / 8) {
+        int64_t share = std::max(cost / slots, floor) * coarser + item;
+        if (n_run <= slots && piece + item <= share + share / 8) {
             for (Tile *x : of) {
                 const int64_t len = x->key1 - x->key0, n = (len + piece - 1) / piece, each = ((len + n - 1) / n + kCut - 1) / kCut * kCut;
                 for (int64_t at = each; at < len; at += each) x->cut.push_back(x->key0 + (int)at);
@@ -226,13 +229,13 @@ std::string attn_plan(const AttnShape &s, int n_cu, int n_seq, const int *q_len,
                 x->fresh = false;
                 for (int at = x->key0;;) {
                     /* no sliver at the end of a run, nor (an eighth over) of a tile */
-                    if (room < kItemCost[kind] + std::min<int64_t>(share / 8, 2 * kCut)) {
+                    if (room < item + std::min<int64_t>(share / 8, 2 * kCut)) {
                         room = share;
                         n_run++;
                         if (at == x->key0) x->fresh = true;
                         else x->cut.push_back(at);
                     }
-                    const int64_t left = x->key1 - at + kItemCost[kind], take = (room - kItemCost[kind] + kCut - 1) / kCut * kCut;
+                    const int64_t left = x->key1 - at + item, take = (room - item + kCut - 1) / kCut * kCut;
                     if (left <= room + share / 8 || at + take >= x->key1) {
                         room -= left;
                         break;
