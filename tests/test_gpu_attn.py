@@ -212,6 +212,19 @@ def test_many_short_sequences(ctx, lens, heads, type_):
     check(np.where(hit, 0, got), np.where(hit, 0, want), np.where(hit, 0, tol))
 
 
+@pytest.mark.parametrize("type_", [F16, F32])
+def test_many_groups_of_few_rows(ctx, type_):
+    """Pairs of sequences on prefixes of their own: shared and own items of few rows, several of them a block."""
+    H = kv = 16
+    runs = [2] * 60
+    b = Batch([(1, 257 + 13 * i % 60) for i in range(120)], 32, shared=256, runs=runs, seed=9)
+    k, v = values(b, kv, 128, type_, 10, shared=256, runs=runs)
+    q = np.random.default_rng(11).standard_normal((b.T, H, 128)).astype(np.float32)
+    print("[case] pairs", flush=True)
+    got = Pool(ctx, H, kv, 128, type_, b).run(q, *pack(b, k, v, kv, 128, type_))
+    check(got, *attend64(b, q, k, v, 128 ** -0.5))
+
+
 def test_scale_and_layers(ctx):
     H, kv, D = 8, 2, 128
     b = Batch([(1, 100), (4, 60)], 32, seed=14)
